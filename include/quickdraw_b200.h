@@ -235,6 +235,77 @@ int qd_batch_attention(const void* qg, const void* k_new, const void* v_new, con
                        const int* positions, int batch, int capacity, int q_heads, int kv_heads,
                        int head_dim, int rotary_dim, float theta, float eps, int splits, void* stream);
 
+/* ---- Paged caches and beam search.  Row p of sequence b is row p mod page of page table[b][p / page] of the pool; sequences may
+ * share pages (refs: how many entries of the table name a page).  An entry that is no page of the pool (-1: none) names rows
+ * that are neither read nor written.  tables int32 [sequences, width]; status: device word, bits are only ever set (a bad
+ * argument on the device: 4; no free page left: 8). */
+
+/* The preparation of qd_batch_attention with the cache rows in pages of [page, kv_heads, head_dim], page_stride elements apart:
+ * norm and RoPE of queries and keys at positions[b], queries to q_out [batch, q_heads, head_dim], key and value rows into the
+ * pool.  head_dim a multiple of 32, rotary_dim of 64. */
+int qd_paged_prepare(const void* qg, const void* k_new, const void* v_new, const void* q_norm, const void* k_norm, void* k_pool,
+                     void* v_pool, long long page_stride, const int* table, void* q_out, const int* positions, int batch,
+                     int width, int pages, int page, int q_heads, int kv_heads, int head_dim, int rotary_dim, float theta,
+                     float eps, void* stream);
+
+/* Attention of one token of every sequence over its first lengths[b] rows (window > 0: over the first `sinks` and the last
+ * `window` of them), query head h on key/value head h / (heads / kv_heads): out [batch, heads, dim] = softmax(scale q k) v,
+ * times sigmoid(gate) where given; zeros for a sequence that sees nothing.  Strides in elements: q and gate by row and head,
+ * the pools (alike) by page, row and head, the table by row.  bf16 or fp32 (is_fp32 = 1); dim at most 256 and a multiple of
+ * 8, pools 16-byte aligned with strides of whole 16-byte pieces, else QD_ERR_UNSUPPORTED.  partial:
+ * qd_paged_attention_floats floats. */
+long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim);
+int qd_paged_attention(const void* q, long long q_row, long long q_head, const void* k, const void* v, long long page_stride,
+                       long long row_stride, long long head_stride, const int* table, long long table_stride,
+                       const int* lengths, const void* gate, long long gate_row, long long gate_head, void* out,
+                       float* partial, int batch, int heads, int kv_heads, int dim, int pages, int page, int width,
+                       int window, int sinks, float scale, int is_fp32, void* stream);
+
+/* scratch of the next three: qd_pages_scratch_words 32-bit words. */
+long long qd_pages_scratch_words(int sequences, int width, int pages);
+
+/* Sequence b goes on as a copy of sequence parents[b], all at once (-1: it ends; itself: it stays as it is).  Full pages are
+ * shared.  A page that is not full goes to the parent itself or else to its first child; the others, in order, get the lowest
+ * free pages and a copy of its rows.  Pools: layers of [page, row], layer_bytes and page_bytes apart, pieces of 16 bytes.
+ * Pages that nobody uses any more keep what they hold.  The outputs are other arrays than the inputs.  Without a free page a
+ * sequence ends where its full pages do (status). */
+int qd_pages_fork(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, int layers,
+                  const int* table, const int* lengths, const int* refs, const int* parents, int* table_out,
+                  int* lengths_out, int* refs_out, int* scratch, unsigned int* status, int sequences, int width, int pages,
+                  int page, void* stream);
+
+/* The pages in use (refs > 0), `used` of them, become the first ones: those behind move, in order, to the free ones in front. */
+int qd_pages_compact(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, int layers,
+                     const int* table, const int* refs, int* table_out, int* refs_out, int* used, int* scratch,
+                     int sequences, int width, int pages, int page, void* stream);
+
+/* Pages for the next counts[b] rows of every sequence (counts NULL: `count`), in place, the lowest free ones in order. */
+int qd_pages_reserve(int* table, const int* lengths, int* refs, const int* counts, int count, int* scratch,
+                     unsigned int* status, int sequences, int width, int pages, int page, void* stream);
+
+/* Rows first .. first + count - 1 of one sequence (table: its row) of every layer from k_rows, v_rows (contiguous rows of
+ * layers rows_layer_bytes apart) to the pool, or (out = 1) from the pool to them. */
+int qd_pages_rows(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, void* k_rows,
+                  void* v_rows, long long rows_layer_bytes, const int* table, unsigned int* status, int layers, int width,
+                  int pages, int page, int first, int count, int out, void* stream);
+
+/* The best `candidates` of scores[b, i] + log_softmax(logits[b, i])[v] over the beams i and tokens v of each group b, the
+ * lowest (i, v) among equals; logits [batch, beams, vocab] bf16 or fp32, rows row_stride elements apart.  A finished beam
+ * (bytes, or NULL) has one continuation, eos, at no cost.  A beam whose score is not finite, or whose logits have no finite
+ * log-sum-exp, has none; what is no continuation counts -inf.  Results [batch, candidates]: fp32 scores, int32 parents
+ * b * beams + i, int64 tokens, best first; placed: a beam's best one in the beam's place, the others in the places left, in
+ * order (candidates == beams).  beams and candidates at most 32.  scratch: qd_beam_scratch_bytes bytes, 8-byte aligned. */
+long long qd_beam_scratch_bytes(int batch, int beams, int vocab, int candidates);
+int qd_beam_select(const void* logits, long long row_stride, int is_fp32, const float* scores, const void* finished, int eos,
+                   float* scores_out, int* parents_out, void* tokens_out, void* scratch, int batch, int beams, int vocab,
+                   int candidates, int placed, void* stream);
+
+/* state[b] = old state[parents[b]] (-1: zeros; itself: not touched) of up to four tensors (NULL: none) of `sequences` rows of
+ * row bytes, stride bytes apart. */
+int qd_reorder_states(void* state0, long long row0, long long stride0, void* state1, long long row1, long long stride1,
+                      void* state2, long long row2, long long stride2, void* state3, long long row3, long long stride3,
+                      const int* parents, unsigned int* status, int sequences, void* stream);
+
 /* The stable order of the chunk's routes by expert (quickdraw/kernel/triton/moe.py:60-97, the
  * grouping the reference builds with a stable sort): ids int32 [routes], every id in
  * [0, experts); order int32 [routes] = route index of each sorted row, boundaries int32

@@ -78,6 +78,17 @@ SIGNATURES = {
     "qd_batch_gdn_recurrence": [P, P, P, P, P, P, L, P, I, I, I, I, I, P],
     "qd_batch_attn_decode": [P, P, P, P, P, P, P, L, P, P, P, P, I, I, I, I, I, I, F, F, I, P],
     "qd_batch_attention": [P, P, P, P, P, P, P, L, P, P, P, P, P, I, I, I, I, I, I, F, F, I, P],
+    "qd_paged_prepare": [P, P, P, P, P, P, P, L, P, P, P, I, I, I, I, I, I, I, I, F, F, P],
+    "qd_paged_attention_floats": [I, I, I, I],
+    "qd_paged_attention": [P, L, L, P, P, L, L, L, P, L, P, P, L, L, P, P, I, I, I, I, I, I, I, I, I, F, I, P],
+    "qd_pages_scratch_words": [I, I, I],
+    "qd_pages_fork": [P, P, L, L, L, I, P, P, P, P, P, P, P, P, P, I, I, I, I, P],
+    "qd_pages_compact": [P, P, L, L, L, I, P, P, P, P, P, P, I, I, I, I, P],
+    "qd_pages_reserve": [P, P, P, P, I, P, P, I, I, I, I, P],
+    "qd_pages_rows": [P, P, L, L, L, P, P, L, P, P, I, I, I, I, I, I, I, P],
+    "qd_beam_scratch_bytes": [I, I, I, I],
+    "qd_beam_select": [P, L, I, P, P, I, P, P, P, P, I, I, I, I, I, P],
+    "qd_reorder_states": [P, L, L, P, L, L, P, L, L, P, L, L, P, P, I, P],
     "qd_seq_group_routes": [P, I, I, P, P, P],
     "qd_seq_moe_combine": [P, P, P, P, P, I, I, I, P],
     "qd_seq_moe_combine_norm": [P, P, P, P, P, P, P, P, I, I, I, F, P],
@@ -136,7 +147,8 @@ STRUCTURES = {"qd_attention_args": AttentionArgs, "qd_latent_args": LatentArgs}
 
 LONG_RESULTS = {"qd_decode_workspace_bytes", "qd_program_bytes", "qd_exchange_bytes",
                 "qd_nvfp4_matmul_rows_scratch_bytes", "qd_seq_gdn_chunk_scratch_bytes",
-                "qd_nvfp4_expert_rows_scratch_bytes"}
+                "qd_nvfp4_expert_rows_scratch_bytes", "qd_paged_attention_floats", "qd_pages_scratch_words",
+                "qd_beam_scratch_bytes"}
 
 _lib = None
 _hybrid: dict[str, ctypes.CDLL] = {}

@@ -12,6 +12,7 @@ weight row once for all sequences; the next token of each sequence is the greedy
 ``BatchState`` stacks the reference's ``DecodeState`` buffers along a leading sequence axis;
 ``sequence(b)`` is a ``DecodeState`` view of one sequence, so a prompt is prefilled with the
 single-sequence chunk prefill and a sequence can be continued by the single-sequence step.
+``PagedBatchState`` (paged.py) has the cache rows in pages that sequences share.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import call, lib, ptr, stream_of
+from .paged import PagedBatchState, paged_attention
 from .prefill import ChunkPrefill
 from .state import DecodeState
 from .weights import Checkpoint
@@ -108,6 +110,8 @@ class BatchDecode(ChunkPrefill):
         c = self.ckpt.config
         batch = x.shape[0]
         qg, k, v = self._matmul_many(x, [w.q_proj, w.k_proj, w.v_proj])
+        if isinstance(state, PagedBatchState):
+            return self._matmul(self._attend_pages(w, qg, k, v, state, index), w.o_proj)
         out = self._empty(batch, c.num_attention_heads * c.head_dim)
         q_scratch = torch.empty_like(out)
         scratch, counters = self._attn_scratch(batch)
@@ -119,14 +123,29 @@ class BatchDecode(ChunkPrefill):
              self._attn_splits(batch, state.max_context), stream_of(x))
         return self._matmul(out, w.o_proj)
 
+    def _attend_pages(self, w, qg, k, v, state: PagedBatchState, index):
+        c, cache = self.ckpt.config, state.cache
+        batch, heads, dim = qg.shape[0], c.num_attention_heads, c.head_dim
+        k_pages, v_pages = cache.k[:, index], cache.v[:, index]
+        q = self._empty(batch, heads, dim)
+        call("qd_paged_prepare", ptr(qg), ptr(k), ptr(v), ptr(w.q_norm), ptr(w.k_norm), ptr(k_pages), ptr(v_pages), k_pages.stride(0), ptr(cache.table),
+             ptr(q), ptr(state.positions), batch, cache.table.shape[1], cache.pages, cache.page, heads, c.num_key_value_heads, dim,
+             int(dim * c.partial_rotary_factor), c.rope_theta, c.rms_norm_eps, stream_of(qg))
+        gate = qg.view(batch, heads, 2 * dim)[:, :, dim:]
+        return paged_attention(q, k_pages, v_pages, cache.table, state.seen, gate=gate).view(batch, heads * dim)
+
     # ------------------------------------------------------------------------------ step
     @torch.inference_mode()
-    def step(self, tokens: torch.Tensor, state: BatchState, *, positions_checked: bool = False):
+    def step(self, tokens: torch.Tensor, state: BatchState | PagedBatchState, *, positions_checked: bool = False):
         """Feed tokens[b] to sequence b at state.positions[b]; advances every position by one."""
         c = self.ckpt.config
         assert tokens.shape == (state.batch,) and tokens.dtype == torch.long and tokens.is_cuda
         if not positions_checked:
             assert int(state.positions.max().item()) < state.max_context, "a sequence has filled its cache"
+        if isinstance(state, PagedBatchState):
+            state.cache.reserve()
+            torch.add(state.positions, 1, out=state.seen)
+            assert positions_checked or state.cache.check() == 0, "the pool has no free page left"
         x = self.ckpt.embed_tokens[tokens].contiguous()
         normed, residual = self._add_norm(x, None, self.gammas[0][0], c.rms_norm_eps)
         # the norm after a layer's MoE block (in front of the next layer, or the final one) rides on its combine
@@ -154,7 +173,7 @@ class BatchDecode(ChunkPrefill):
         call("qd_argmax_rows", ptr(logits), state.batch, logits.shape[1], ptr(picked), stream_of(logits))
         return picked, logits
 
-    def graph_step(self, tokens: torch.Tensor, state: BatchState):
+    def graph_step(self, tokens: torch.Tensor, state: BatchState | PagedBatchState):
         """``step`` replayed from a CUDA graph: a step is some 1 100 launches, which the host
         issues more slowly than the GPU runs them.  The first call with a state runs eagerly (it
         also loads and configures every kernel), the second captures, later ones replay; the
@@ -187,6 +206,6 @@ class BatchDecode(ChunkPrefill):
         entry["bound"] += 1
         return entry["out"]
 
-    def forget(self, state: BatchState) -> None:
+    def forget(self, state: BatchState | PagedBatchState) -> None:
         """Drop the captured graph of a state (its positions were written from outside)."""
         self._graphs.pop(id(state), None)

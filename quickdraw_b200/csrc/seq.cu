@@ -666,7 +666,8 @@ __global__ void seq_attn_prepare_kernel(const bf16* __restrict__ qg, const bf16*
                                         const bf16* __restrict__ k_norm, bf16* __restrict__ k_cache,
                                         bf16* __restrict__ v_cache, bf16* __restrict__ q_out, int position0, int hq,
                                         int hk, int d, int rotary, float theta, float eps,
-                                        const int* __restrict__ positions, long long cache_stride, int capacity) {
+                                        const int* __restrict__ positions, long long cache_stride, int capacity,
+                                        const int* __restrict__ table, int width, int pages, int page) {
     chain_enter();
     const int t = blockIdx.y, head = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (head >= hq + hk) return;
@@ -674,8 +675,14 @@ __global__ void seq_attn_prepare_kernel(const bf16* __restrict__ qg, const bf16*
     // sequence t at its own position in its own cache
     const int position = positions ? positions[t] : position0 + t;
     if (position < 0 || position >= capacity) return;      // a position outside the cache touches nothing
-    if (positions) { k_cache += (size_t)t * cache_stride; v_cache += (size_t)t * cache_stride; }
     const bool is_q = head < hq;
+    size_t row = position;
+    if (table) {           // rows in pages, cache_stride elements apart
+        const int entry = table[(size_t)t * width + position / page];
+        if (!is_q && (entry < 0 || entry >= pages)) return;
+        if (!is_q) { k_cache += entry * cache_stride; v_cache += entry * cache_stride; }
+        row = position % page;
+    } else if (positions) { k_cache += (size_t)t * cache_stride; v_cache += (size_t)t * cache_stride; }
     const bf16* src = is_q ? qg + ((size_t)t * hq + head) * 2 * d : k_new + ((size_t)t * hk + (head - hq)) * d;
     const bf16* gamma_w = is_q ? q_norm : k_norm;
     float v[8], g[8];
@@ -704,7 +711,7 @@ __global__ void seq_attn_prepare_kernel(const bf16* __restrict__ qg, const bf16*
             v[j + hj] = round_bf16(hi * c + lo * sn);
         }
     }
-    bf16* dst = is_q ? q_out + ((size_t)t * hq + head) * d : k_cache + ((size_t)position * hk + (head - hq)) * d;
+    bf16* dst = is_q ? q_out + ((size_t)t * hq + head) * d : k_cache + (row * hk + (head - hq)) * d;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int i = j * 32 + lane;
@@ -712,7 +719,7 @@ __global__ void seq_attn_prepare_kernel(const bf16* __restrict__ qg, const bf16*
     }
     if (!is_q) {
         const bf16* vs = v_new + ((size_t)t * hk + (head - hq)) * d;
-        bf16* vd = v_cache + ((size_t)position * hk + (head - hq)) * d;
+        bf16* vd = v_cache + (row * hk + (head - hq)) * d;
         for (int i = lane; i < d; i += 32) vd[i] = vs[i];
     }
 }
@@ -1703,7 +1710,7 @@ extern "C" int qd_seq_attention(const void* qg, const void* k_new, const void* v
     qd_launch(seq_attn_prepare_kernel, dim3((heads + 7) / 8, tokens), dim3(256), 0, (cudaStream_t)stream, true, 
         (const bf16*)qg, (const bf16*)k_new, (const bf16*)v_new, (const bf16*)q_norm, (const bf16*)k_norm,
         (bf16*)k_cache, (bf16*)v_cache, (bf16*)q_scratch, position0, q_heads, kv_heads, head_dim, rotary_dim, theta, eps,
-        nullptr, 0, capacity);
+        nullptr, 0, capacity, nullptr, 0, 0, 1);
     if (qd_launch_status() != QD_OK) return QD_ERR_LAUNCH;
     // Tensor cores but for the first few positions of a sequence, where the walk of a position at a time is over sooner (both with the
     // preparation, 16/2 heads): 24 tokens at position 0 16 against 23 us, 33 21 against 24, 64 35 against 24; 23 at position 20 23 against
@@ -1739,7 +1746,7 @@ extern "C" int qd_batch_attention(const void* qg, const void* k_new, const void*
     qd_launch(seq_attn_prepare_kernel, dim3((heads + 7) / 8, batch), dim3(256), 0, (cudaStream_t)stream, true, 
         (const bf16*)qg, (const bf16*)k_new, (const bf16*)v_new, (const bf16*)q_norm, (const bf16*)k_norm,
         (bf16*)k_cache, (bf16*)v_cache, (bf16*)q_scratch, 0, q_heads, kv_heads, head_dim, rotary_dim, theta, eps,
-        positions, cache_stride, capacity);
+        positions, cache_stride, capacity, nullptr, 0, 0, 1);
     if (qd_launch_status() != QD_OK) return QD_ERR_LAUNCH;
     LaneAttnParams p;
     p.q = (const bf16*)q_scratch; p.qg = (const bf16*)qg; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;
@@ -1784,6 +1791,19 @@ extern "C" int qd_batch_attention(const void* qg, const void* k_new, const void*
     }
     qd_launch(batch_attn_lanes_kernel, dim3(kv_heads, splits, batch), dim3(kLaneAttnWarps * 32), smem, (cudaStream_t)stream, true, p);
     return qd_launch_status();
+}
+
+/* the preparation alone, with the caches' rows in pages */
+extern "C" int qd_paged_prepare(const void* qg, const void* k_new, const void* v_new, const void* q_norm, const void* k_norm, void* k_pool, void* v_pool,
+                                long long page_stride, const int* table, void* q_out, const int* positions, int batch, int width, int pages, int page,
+                                int q_heads, int kv_heads, int head_dim, int rotary_dim, float theta, float eps, void* stream) {
+    QD_CHECK_ARG(qg && k_new && v_new && q_norm && k_norm && k_pool && v_pool && table && q_out && positions);
+    QD_CHECK_ARG(batch > 0 && batch <= 65535 && width > 0 && pages > 0 && page > 0 && (long long)width * page <= 0x7fffffffll);
+    QD_CHECK_ARG(kv_heads > 0 && q_heads % kv_heads == 0 && page_stride >= (long long)page * kv_heads * head_dim);
+    if (head_dim > 256 || head_dim % 32 != 0 || rotary_dim % 64 != 0 || rotary_dim > head_dim) return QD_ERR_UNSUPPORTED;
+    return qd_launch(seq_attn_prepare_kernel, dim3((q_heads + kv_heads + 7) / 8, batch), dim3(256), 0, (cudaStream_t)stream, true,
+        (const bf16*)qg, (const bf16*)k_new, (const bf16*)v_new, (const bf16*)q_norm, (const bf16*)k_norm, (bf16*)k_pool, (bf16*)v_pool, (bf16*)q_out, 0,
+        q_heads, kv_heads, head_dim, rotary_dim, theta, eps, positions, page_stride, width * page, table, width, pages, page);
 }
 
 extern "C" int qd_argmax_rows(const void* logits, int rows, int columns, void* tokens, void* stream) {

@@ -1,0 +1,179 @@
+"""Refusals of the paged cache's and the beams' entry points, and what their drivers pass on, without a GPU."""
+
+import math
+
+import pytest
+import torch
+
+from quickdraw_b200 import _lib, beam, paged, synthetic
+from tests import paged_plain as plain
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+class AsIfOnGpu(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
+
+def on_gpu(t):
+    return t.as_subclass(AsIfOnGpu)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library replaced by a recorder that knows how many arguments each entry point takes."""
+    seen = []
+
+    def record(name, *args):
+        assert len(args) == len(_lib.SIGNATURES[name]), (name, len(args), len(_lib.SIGNATURES[name]))
+        seen.append((name, args))
+
+    monkeypatch.setattr(paged, "call", record)
+    monkeypatch.setattr(paged, "stream_of", lambda t: None)
+    return seen
+
+
+def attention_arguments(**changes):
+    given = dict(q=torch.zeros(2, 16, 256, dtype=BF16), k_pages=torch.zeros(9, 16, 2, 256, dtype=BF16), v_pages=torch.zeros(9, 16, 2, 256, dtype=BF16),
+                 table=torch.zeros(2, 5, dtype=I32), lengths=torch.zeros(2, dtype=I32)) | changes
+    return {name: on_gpu(t) if isinstance(t, torch.Tensor) else t for name, t in given.items()}
+
+
+def test_attention_passes_its_arguments(calls):
+    out = paged.paged_attention(**attention_arguments())
+    assert out.shape == (2, 16, 256) and out.dtype is BF16 and [name for name, _ in calls] == ["qd_paged_attention"]
+    args = calls[0][1]
+    assert args[1:3] == (16 * 256, 256) and args[5:8] == (16 * 2 * 256, 2 * 256, 256) and args[16:25] == (2, 16, 2, 256, 9, 16, 5, 0, 0)
+    assert args[25] == 1 / 16 and args[26] == 0
+
+
+@pytest.mark.parametrize("changes", [
+    dict(q=torch.zeros(2, 16, 256, dtype=torch.float16)), dict(q=torch.zeros(16, 256, dtype=BF16)), dict(q=torch.zeros(2, 15, 256, dtype=BF16)),
+    dict(q=torch.zeros(2, 16, 256)), dict(q=torch.zeros(3, 16, 256, dtype=BF16)), dict(q=torch.zeros(2, 256, 16, dtype=BF16).transpose(1, 2)),
+    dict(q=torch.zeros(0, 16, 256, dtype=BF16), table=torch.zeros(0, 5, dtype=I32), lengths=torch.zeros(0, dtype=I32)),
+    dict(q=torch.zeros(2, 16, 264, dtype=BF16), k_pages=torch.zeros(9, 16, 2, 264, dtype=BF16), v_pages=torch.zeros(9, 16, 2, 264, dtype=BF16)),
+    dict(q=torch.zeros(2, 16, 12, dtype=BF16), k_pages=torch.zeros(9, 16, 2, 12, dtype=BF16), v_pages=torch.zeros(9, 16, 2, 12, dtype=BF16)),
+    dict(k_pages=torch.zeros(9, 16, 2, 256)), dict(v_pages=torch.zeros(8, 16, 2, 256, dtype=BF16)), dict(k_pages=torch.zeros(9, 2, 256, dtype=BF16)),
+    dict(k_pages=torch.zeros(9, 2, 16, 256, dtype=BF16).transpose(1, 2)), dict(k_pages=torch.zeros(0, 16, 2, 256, dtype=BF16), v_pages=torch.zeros(0, 16, 2, 256, dtype=BF16)),
+    dict(k_pages=torch.zeros(9 * 16 * 2 * 256 + 1, dtype=BF16)[1:].view(9, 16, 2, 256)),
+    dict(table=torch.zeros(2, 5, dtype=torch.long)), dict(table=torch.zeros(3, 5, dtype=I32)), dict(table=torch.zeros(2, 0, dtype=I32)),
+    dict(table=torch.zeros(5, 2, dtype=I32).T), dict(lengths=torch.zeros(3, dtype=I32)), dict(lengths=torch.zeros(2)), dict(window=-1), dict(sinks=3),
+    dict(window=3, sinks=-1), dict(gate=torch.zeros(2, 16, 256)), dict(gate=torch.zeros(2, 16, 128, dtype=BF16))])
+def test_attention_refuses(calls, changes):
+    with pytest.raises(AssertionError):
+        paged.paged_attention(**attention_arguments(**changes))
+    assert not calls
+
+
+def test_attention_refuses_the_cpu(calls):
+    given = attention_arguments()
+    with pytest.raises(AssertionError, match="CUDA"):
+        paged.paged_attention(**{name: t.as_subclass(torch.Tensor) for name, t in given.items()})
+
+
+def page_arguments(**changes):
+    given = dict(k_pages=torch.zeros(9, 3, 16, 2, 64, dtype=BF16), v_pages=torch.zeros(9, 3, 16, 2, 64, dtype=BF16), table=torch.zeros(4, 5, dtype=I32),
+                 lengths=torch.zeros(4, dtype=I32), refs=torch.zeros(9, dtype=I32), parents=torch.zeros(4, dtype=I32), status=torch.zeros(1, dtype=I32)) | changes
+    return {name: on_gpu(t) for name, t in given.items()}
+
+
+def test_forks_and_compactions_pass_their_arguments(calls):
+    given = page_arguments()
+    out = paged.fork_pages(**given)
+    assert [t.shape for t in out] == [(4, 5), (4,), (9,)]
+    assert calls[-1][0] == "qd_pages_fork" and calls[-1][1][2:6] == (3 * 16 * 256, 16 * 256, 256, 3) and calls[-1][1][15:19] == (4, 5, 9, 16)
+    out = paged.compact_pages(*(given[name] for name in ("k_pages", "v_pages", "table", "refs")))
+    assert [t.shape for t in out] == [(4, 5), (9,), ()] and calls[-1][0] == "qd_pages_compact"
+    paged.reserve_pages(given["table"], given["lengths"], given["refs"], 16, 3, status=given["status"])
+    assert calls[-1][0] == "qd_pages_reserve" and calls[-1][1][3:5] == (None, 3)
+    paged.reserve_pages(given["table"], given["lengths"], given["refs"], 16, given["lengths"], status=given["status"])
+    assert calls[-1][1][4] == 0
+
+
+@pytest.mark.parametrize("changes", [
+    dict(k_pages=torch.zeros(9, 16, 2, 64, dtype=BF16)), dict(k_pages=torch.zeros(9, 3, 16, 2, 64)), dict(k_pages=torch.zeros(9, 2, 16, 2, 64, dtype=BF16)),
+    dict(k_pages=torch.zeros(9, 16, 3, 2, 64, dtype=BF16).transpose(1, 2)),
+    dict(k_pages=torch.zeros(9, 3, 16, 1, 4, dtype=BF16), v_pages=torch.zeros(9, 3, 16, 1, 4, dtype=BF16)), dict(refs=torch.zeros(8, dtype=I32)),
+    dict(refs=torch.zeros(9)), dict(table=torch.zeros(4, 5)), dict(table=torch.zeros(4, 10, dtype=I32)[:, ::2]), dict(lengths=torch.zeros(5, dtype=I32)),
+    dict(parents=torch.zeros(4, dtype=torch.long)), dict(parents=torch.zeros(3, dtype=I32)), dict(status=torch.zeros(2, dtype=I32))])
+def test_forks_refuse(calls, changes):
+    with pytest.raises(AssertionError):
+        paged.fork_pages(**page_arguments(**changes))
+    assert not calls
+
+
+def test_reserves_refuse(calls):
+    table, lengths, refs, status = (on_gpu(torch.zeros(*shape, dtype=I32)) for shape in ((4, 5), (4,), (9,), (1,)))
+    for page, counts in ((0, 1), (16, -1), (16, torch.zeros(4)), (16, torch.zeros(3, dtype=I32)), (2 ** 30, 1)):
+        with pytest.raises(AssertionError):
+            paged.reserve_pages(table, lengths, refs, page, counts, status=status)
+    assert not calls
+
+
+def test_cache_of_no_size_is_refused():
+    for sizes in ((0, 2, 64, 4, 16, 2, 100), (1, 2, 64, 0, 16, 2, 100), (1, 2, 64, 4, 0, 2, 100), (1, 2, 64, 4, 16, 0, 100), (1, 2, 64, 4, 16, 2, 0)):
+        with pytest.raises(AssertionError):
+            paged.PagedCache(*sizes, "cpu")
+    cache = paged.PagedCache(2, 2, 64, 4, 16, 3, 100, "cpu")
+    assert cache.table.shape == (3, 7) and bool((cache.table == -1).all()) and cache.pages == 4 and cache.check() == 0
+    with pytest.raises(AssertionError):
+        cache.free([3])
+
+
+def test_select_passes_its_arguments(calls):
+    logits, scores = on_gpu(torch.zeros(2, 3, 50)), on_gpu(torch.zeros(2, 3))
+    out = beam.beam_select(logits, scores)
+    assert [(t.shape, t.dtype) for t in out] == [((2, 3), F32), ((2, 3), I32), ((2, 3), torch.long)]
+    assert calls[-1][0] == "qd_beam_select" and calls[-1][1][1:3] == (50, 1) and calls[-1][1][10:15] == (2, 3, 50, 3, 1)
+    out = beam.beam_select(logits, scores, candidates=6, finished=on_gpu(torch.zeros(2, 3, dtype=torch.bool)), eos=49)
+    assert out[0].shape == (2, 6) and calls[-1][1][5] == 49 and calls[-1][1][13:15] == (6, 0)
+
+
+@pytest.mark.parametrize("logits,scores,kwargs", [
+    (torch.zeros(2, 3, 50, dtype=torch.float16), torch.zeros(2, 3), {}), (torch.zeros(6, 50), torch.zeros(2, 3), {}), (torch.zeros(2, 33, 50), torch.zeros(2, 33), {}),
+    (torch.zeros(2, 3, 50), torch.zeros(3, 2), {}), (torch.zeros(2, 3, 50), torch.zeros(2, 3, dtype=BF16), {}), (torch.zeros(2, 50, 3).transpose(1, 2), torch.zeros(2, 3), {}),
+    (torch.zeros(3, 2, 50).transpose(0, 1), torch.zeros(2, 3), {}), (torch.zeros(2, 3, 50), torch.zeros(2, 3), dict(candidates=0)),
+    (torch.zeros(2, 3, 50), torch.zeros(2, 3), dict(candidates=33)), (torch.zeros(2, 3, 5), torch.zeros(2, 3), dict(candidates=16)),
+    (torch.zeros(2, 3, 50), torch.zeros(2, 3), dict(finished=torch.zeros(2, 3, dtype=torch.bool))),
+    (torch.zeros(2, 3, 50), torch.zeros(2, 3), dict(finished=torch.zeros(2, 3, dtype=torch.bool), eos=50)),
+    (torch.zeros(2, 3, 50), torch.zeros(2, 3), dict(finished=torch.zeros(2, 3), eos=5)), (torch.zeros(0, 3, 50), torch.zeros(0, 3), {}),
+    (torch.zeros(2, 3, 0), torch.zeros(2, 3), {})])
+def test_select_refuses(calls, logits, scores, kwargs):
+    with pytest.raises(AssertionError):
+        beam.beam_select(on_gpu(logits), on_gpu(scores), **{name: on_gpu(t) if isinstance(t, torch.Tensor) else t for name, t in kwargs.items()})
+    assert not calls
+
+
+def test_reorder_passes_its_arguments_and_refuses(calls):
+    parents, status = on_gpu(torch.zeros(3, dtype=I32)), on_gpu(torch.zeros(1, dtype=I32))
+    beam.reorder_states([on_gpu(torch.zeros(3, 4)) for _ in range(6)], parents, status=status)
+    assert [len(args) for _, args in calls] == [16, 16] and calls[1][1][6] is None and calls[0][1][1:3] == (16, 16)
+    calls.clear()
+    for state in (torch.zeros(4, 4), torch.zeros(3, 4, 4).transpose(1, 2), torch.zeros(1, 4).expand(3, 4), torch.zeros(())):
+        with pytest.raises(AssertionError):
+            beam.reorder_states(on_gpu(state), parents, status=status)
+    with pytest.raises(AssertionError):
+        beam.reorder_states(on_gpu(torch.zeros(3, 4)), on_gpu(torch.zeros(3, dtype=torch.long)), status=status)
+    assert not calls
+
+
+def test_search_refuses():
+    class Decoder:
+        class ckpt:
+            config = synthetic.model_config(num_layers=4, vocab_size=64)
+        device = "cpu"
+    for prompts, beams, tokens, kwargs in (([], 2, 3, {}), ([[]], 2, 3, {}), ([[1]], 0, 3, {}), ([[1]], 33, 3, {}), ([[64]], 2, 3, {}), ([[1]], 2, -1, {}),
+                                           ([[1]], 2, 3, dict(eos=64))):
+        with pytest.raises(AssertionError):
+            beam.beam_search(Decoder, prompts, beams, tokens, **kwargs)
+    assert beam.beam_search(Decoder, [[1], [2]], 2, 0) == [[([], 0.0)], [([], 0.0)]]
+
+
+def test_plain_forms_agree_with_themselves():
+    """The oracle's fork keeps every sequence's rows and counts every entry; its attention of a forked sequence is its parent's."""
+    k, v, table, lengths, refs = plain.cache([37, 5, 0, 16], 16, 1, 2, 8, F32, seed=1, spare=6, device="cpu")
+    new = plain.fork(k, v, table, lengths, refs, [0, 0, 1, 0], 16)
+    assert new[5] == 0 and new[3].tolist() == [37, 37, 5, 37] and int(new[4].sum()) == int((new[2] >= 0).sum())
+    q = torch.randn(4, 2, 8, generator=torch.Generator().manual_seed(1))[:1].expand(4, 2, 8)
+    out, bound = plain.attention(q, new[0][:, 0], new[1][:, 0], new[2], new[3])
+    assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[3]) and not math.isnan(float(out.sum())) and float(bound.max()) < 1e-2
