@@ -1,78 +1,10 @@
 // Attention of one new token of every sequence over keys and values in pages:
 //   out[b, h] = sum_p softmax_p(scale q[b, h] . k[p]) v[p],   row p of sequence b in pool[table[b][p / page]][p mod page],
 // over the positions p that the sequence sees (all, or the first few and a window), times sigmoid(gate) where given.
-#include "paged.cuh"
-
-#include <type_traits>
+#include "paged_mma.cuh"
 
 namespace qd {
 namespace {
-
-template <typename T> QD_DEVINL float paged_load(const T* p) { return (float)*p; }
-template <> QD_DEVINL float paged_load<bf16>(const bf16* p) { return __bfloat162float(*p); }
-template <typename T> QD_DEVINL void paged_store(T* p, float v);
-template <> QD_DEVINL void paged_store<float>(float* p, float v) { *p = v; }
-template <> QD_DEVINL void paged_store<bf16>(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-constexpr int kSeqs = 1024;             // sequences of a launch
-
-// The sequences' parts, in front of one another: before[b] pieces (a part of a pair each) belong to the sequences below b.
-template <int THREADS>
-QD_DEVINL int paged_schedule(const PagedParams& p, int* before) {
-    __shared__ int sums[THREADS / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = p.kv_heads * p.chunks;
-    int total = 0;
-    for (int base = 0; base < p.batch; base += THREADS) {
-        const int b = base + tid;
-        int sum = b < p.batch ? each * paged_parts(paged_span(p, b).seen, p.unit, (long long)p.batch * each, (int)gridDim.x) : 0;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += up;
-        }
-        if (lane == 31) sums[warp] = sum;
-        __syncthreads();
-        int all = 0;
-        for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) sum += sums[w]; all += sums[w]; }
-        if (b < p.batch) before[b + 1] = total + sum;
-        total += all;
-        __syncthreads();
-    }
-    if (tid == 0) before[0] = 0;
-    __syncthreads();
-    return total;
-}
-
-struct Piece { int b, kvh, head0, heads, t0, t1, skip, part, parts; long long pair; };
-QD_DEVINL Piece paged_piece(const PagedParams& p, const int* before, int r) {
-    int lo = 0;
-    for (int hi = p.batch; hi - lo > 1;) {
-        const int mid = (lo + hi) >> 1;
-        if (before[mid] <= r) lo = mid; else hi = mid;
-    }
-    Piece a;
-    const int each = p.kv_heads * p.chunks;
-    const Span s = paged_span(p, lo);
-    a.b = lo;
-    a.parts = (before[lo + 1] - before[lo]) / each;
-    const int at = r - before[lo], pair = at / a.parts, units = (s.seen + p.unit - 1) / p.unit;
-    a.part = at - pair * a.parts;
-    a.kvh = pair / p.chunks;
-    const int chunk = pair - a.kvh * p.chunks;
-    a.head0 = a.kvh * p.group + chunk * p.chunk;
-    a.heads = min(p.chunk, p.group - chunk * p.chunk);
-    a.pair = (long long)lo * each + pair;
-    a.t0 = min(s.seen, (int)((long long)units * a.part / a.parts) * p.unit);
-    a.t1 = min(s.seen, (int)((long long)units * (a.part + 1) / a.parts) * p.unit);
-    a.skip = s.skip;
-    return a;
-}
-
-template <typename T>
-QD_DEVINL void paged_put(const PagedParams& p, int b, int head, int f, float v) {
-    if (p.gate) v *= sigmoid_precise(paged_load((const T*)p.gate + b * p.gate_row + head * p.gate_head + f));
-    paged_store((T*)p.out + ((long long)b * p.heads + head) * p.dim + f, v);
-}
 
 // A warp per position, a lane for every 32nd feature, fp32 sums.
 constexpr int kPlainWarps = 8, kPlainHeads = 8;
@@ -80,11 +12,11 @@ template <typename T>
 __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const PagedParams p) {
     chain_enter();
     extern __shared__ __align__(16) float plain_smem[];                // [warps][heads][dim + 2]
-    __shared__ int before[kSeqs + 1];
+    __shared__ int before[kPagedSeqs + 1], seen[kPagedSeqs];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = p.dim + 2;
-    const int total = paged_schedule<kPlainWarps * 32>(p, before);
+    const int total = paged_schedule<kPlainWarps * 32>(p, before, seen);
     for (int r = blockIdx.x; r < total; r += gridDim.x) {
-        const Piece a = paged_piece(p, before, r);
+        const Piece a = paged_piece(p, before, seen, r);
         float q[kPlainHeads][8], acc[kPlainHeads][8], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
         for (int h = 0; h < kPlainHeads; ++h) {
@@ -141,7 +73,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const Pag
             }
             if (a.parts == 1) paged_put<T>(p, a.b, a.head0 + h, f, den == 0.f ? 0.f : num / den);
             else {
-                float* dst = p.partial + ((a.pair * p.most + a.part) * p.chunk + h) * stride;
+                float* dst = p.partial + (((long long)a.pair * p.most + a.part) * p.chunk + h) * stride;
                 dst[f] = num;
                 if (f == 0) { dst[p.dim] = top; dst[p.dim + 1] = den; }
             }
@@ -150,27 +82,52 @@ __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const Pag
     }
 }
 
-// The parts of a (sequence, head) joined; a sequence that sees nothing gets zeros.
+// The parts of a (sequence, head) joined, a warp for every eighth part; a sequence that sees nothing gets zeros.
+constexpr int kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, int blocks) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int blocks) {
     chain_enter();
-    const int head = blockIdx.x, b = blockIdx.y, each = p.kv_heads * p.chunks;
+    __shared__ float state[kJoinWarps][256 + 2];
+    const int head = blockIdx.x, b = blockIdx.y, each = p.kv_heads * p.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int parts = paged_parts(paged_span(p, b).seen, p.unit, (long long)p.batch * each, blocks);
     if (parts == 1) return;
     const int kvh = head / p.group, in = head - kvh * p.group, stride = p.dim + 2;
-    const long long pair = (long long)b * each + kvh * p.chunks + in / p.chunk;
+    const long long pair = (long long)b * each + kvh * p.chunks + in / p.chunk, step = (long long)p.chunk * stride;
     const float* src = p.partial + (pair * p.most * p.chunk + in % p.chunk) * stride;
-    const long long step = (long long)p.chunk * stride;
-    for (int f = threadIdx.x; f < p.dim; f += blockDim.x) {
-        float top = -INFINITY, num = 0.f, den = 0.f;
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, src[i * step + p.dim]);
-        for (int i = 0; i < parts; ++i) {
-            const float g = src[i * step + p.dim + 1] == 0.f ? 0.f : exp2f(src[i * step + p.dim] - top);
-            num += g * src[i * step + f];
-            den += g * src[i * step + p.dim + 1];
+    float top = -INFINITY, den = 0.f, num[8] = {};
+    for (int base = warp; base < parts; base += 32 * kJoinWarps) {
+        const int mine = base + lane * kJoinWarps;                     // a lane's part
+        const float m = mine < parts ? src[mine * step + p.dim] : -INFINITY, l = mine < parts ? src[mine * step + p.dim + 1] : 0.f;
+        const float now = fmaxf(top, warp_max(m)), shift = now == -INFINITY ? 0.f : now, fix = exp2f(top - shift), w = l == 0.f ? 0.f : exp2f(m - shift);
+        top = now;
+        den = den * fix + warp_sum(w * l);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) num[j] *= fix;
+        const int count = min(32, (parts - base + kJoinWarps - 1) / kJoinWarps);
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float each_w = __shfl_sync(0xffffffffu, w, i);
+            const float* row = src + (base + i * kJoinWarps) * step;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j * 32 + lane < p.dim) num[j] += each_w * row[j * 32 + lane];
         }
-        paged_put<T>(p, b, head, f, den == 0.f ? 0.f : num / den);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) state[warp][j * 32 + lane] = num[j];
+    if (lane == 0) { state[warp][256] = top; state[warp][257] = den; }
+    __syncthreads();
+    if (tid >= p.dim) return;
+    float all = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, state[w][256]);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float g = state[w][257] == 0.f ? 0.f : exp2f(state[w][256] - all);
+        sum += g * state[w][257];
+        v += g * state[w][tid];
+    }
+    paged_put<T>(p, b, head, tid, sum == 0.f ? 0.f : v / sum);
 }
 
 int paged_blocks() {
@@ -178,16 +135,34 @@ int paged_blocks() {
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     return sms > 0 ? sms : 148;
 }
-int chunk_of(int group) { return group < kPlainHeads ? group : kPlainHeads; }
+// Query heads at a time: eight columns of a tensor-core instruction, or twice as many on the same keys and values.
+int chunk_of(int group, bool fp32) {
+    const int most = fp32 || group <= 8 ? 8 : 16;
+    return group < most ? group : most;
+}
+int unit_of(int dim, bool fp32) { return fp32 ? 32 : dim <= 64 ? 256 : dim <= 128 ? 128 : 64; }         // a tile for each warp
 
-template <typename T>
-int paged_launch(PagedParams p, cudaStream_t stream) {
-    const int blocks = paged_blocks();
+template <int D, int NT>
+int mma_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
+    constexpr int kSmem = PagedMma<D, NT>::kSmem;
+    if (cudaFuncSetAttribute(paged_mma_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return QD_ERR_LAUNCH;
+    return qd_launch(paged_mma_kernel<D, NT>, dim3(blocks), dim3(PagedMma<D, NT>::kThreads), kSmem, stream, 3, p);
+}
+int plain_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
     const size_t smem = sizeof(float) * kPlainWarps * kPlainHeads * (p.dim + 2);
-    if (cudaFuncSetAttribute(paged_plain_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
-    int code = qd_launch(paged_plain_kernel<T>, dim3(blocks), dim3(kPlainWarps * 32), smem, stream, 3, p);
-    if (code == QD_OK) code = qd_launch(paged_join_kernel<T>, dim3(p.heads, p.batch), dim3(p.dim < 256 ? (p.dim + 31) / 32 * 32 : 256), 0, stream, 3, p, blocks);
-    return code;
+    if (cudaFuncSetAttribute(paged_plain_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
+    return qd_launch(paged_plain_kernel<float>, dim3(blocks), dim3(kPlainWarps * 32), smem, stream, 3, p);
+}
+int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
+    const int blocks = paged_blocks();
+    const bool two = p.chunk > 8;
+    int code = fp32 ? plain_launch(p, blocks, stream)
+             : p.dim <= 64 ? (two ? mma_launch<64, 2>(p, blocks, stream) : mma_launch<64, 1>(p, blocks, stream))
+             : p.dim <= 128 ? (two ? mma_launch<128, 2>(p, blocks, stream) : mma_launch<128, 1>(p, blocks, stream))
+                            : (two ? mma_launch<256, 2>(p, blocks, stream) : mma_launch<256, 1>(p, blocks, stream));
+    if (code != QD_OK) return code;
+    const dim3 grid(p.heads, p.batch), block(kJoinWarps * 32);
+    return fp32 ? qd_launch(paged_join_kernel<float>, grid, block, 0, stream, 3, p, blocks) : qd_launch(paged_join_kernel<bf16>, grid, block, 0, stream, 3, p, blocks);
 }
 
 }  // namespace
@@ -197,11 +172,15 @@ using namespace qd;
 
 extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim) {
     if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
-    const int group = heads / kv_heads, chunk = chunk_of(group), chunks = (group + chunk - 1) / chunk, few = batch < kSeqs ? batch : kSeqs;
-    const long long pairs = (long long)few * kv_heads * chunks, rest = (long long)(batch % kSeqs) * kv_heads * chunks;
-    const int blocks = paged_blocks();
-    const long long whole = pairs * paged_most(pairs, blocks), last = batch > kSeqs && rest ? rest * paged_most(rest, blocks) : 0;
-    return (whole > last ? whole : last) * chunk * (dim + 2);
+    const int group = heads / kv_heads, blocks = paged_blocks();
+    long long most = 0;
+    for (int fp32 = 0; fp32 < 2; ++fp32)
+        for (const int some : {batch < kPagedSeqs ? batch : kPagedSeqs, batch % kPagedSeqs}) {          // whole launches and the last one
+            const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
+            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_most(pairs, blocks) * chunk * (dim + 2);
+            if (floats > most) most = floats;
+        }
+    return most;
 }
 
 extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_head, const void* k, const void* v, long long page_stride,
@@ -216,18 +195,22 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     p.q_row = q_row; p.q_head = q_head; p.gate_row = gate_row; p.gate_head = gate_head;
     p.page_stride = page_stride; p.row_stride = row_stride; p.head_stride = head_stride; p.table_stride = table_stride;
     p.k = k; p.v = v; p.partial = partial;
-    p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pages = pages; p.page = page; p.width = width; p.window = window; p.sinks = sinks;
-    p.group = heads / kv_heads; p.chunk = chunk_of(p.group); p.chunks = (p.group + p.chunk - 1) / p.chunk;
-    p.unit = 32; p.scale = scale * 1.4426950408889634f;
+    p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pages = pages; p.page = page; p.width = width;
+    const bool all = (long long)window + sinks >= (long long)width * page;      // (their sum fits 32 bits otherwise)
+    p.window = all ? 0 : window; p.sinks = all ? 0 : sinks;
+    p.group = heads / kv_heads; p.chunk = chunk_of(p.group, is_fp32); p.chunks = (p.group + p.chunk - 1) / p.chunk;
+    p.unit = unit_of(dim, is_fp32); p.scale = scale * 1.4426950408889634f;
     const int size = is_fp32 ? 4 : 2;
-    for (int b = 0; b < batch; b += kSeqs) {                 // (the scratch is used again in stream order)
-        p.batch = batch - b < kSeqs ? batch - b : kSeqs;
+    p.q_whole = !(((uintptr_t)q | (uintptr_t)(q_row * size) | (uintptr_t)(q_head * size)) & 15u);
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(page_stride * size) | (uintptr_t)(row_stride * size) | (uintptr_t)(head_stride * size)) & 15u) return QD_ERR_UNSUPPORTED;
+    for (int b = 0; b < batch; b += kPagedSeqs) {                 // (the scratch is used again in stream order)
+        p.batch = batch - b < kPagedSeqs ? batch - b : kPagedSeqs;
         p.most = paged_most((long long)p.batch * kv_heads * p.chunks, paged_blocks());
         p.q = (const char*)q + b * q_row * size;
         p.gate = gate ? (const char*)gate + b * gate_row * size : nullptr;
         p.out = (char*)out + (long long)b * heads * dim * size;
         p.table = table + b * table_stride; p.lengths = lengths + b;
-        const int code = is_fp32 ? paged_launch<float>(p, (cudaStream_t)stream) : paged_launch<bf16>(p, (cudaStream_t)stream);
+        const int code = paged_launch(p, is_fp32 != 0, (cudaStream_t)stream);
         if (code != QD_OK) return code;
     }
     return QD_OK;
