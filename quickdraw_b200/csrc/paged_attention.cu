@@ -12,11 +12,11 @@ template <typename T>
 __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const PagedParams p) {
     chain_enter();
     extern __shared__ __align__(16) float plain_smem[];                // [warps][heads][dim + 2]
-    __shared__ int before[kPagedSeqs + 1], seen[kPagedSeqs];
+    __shared__ PagedOrder order;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = p.dim + 2;
-    const int total = paged_schedule<kPlainWarps * 32>(p, before, seen);
-    for (int r = blockIdx.x; r < total; r += gridDim.x) {
-        const Piece a = paged_piece(p, before, seen, r);
+    const int total = paged_schedule<kPlainWarps * 32>(p, order, (int)gridDim.x);
+    for (int r = blockIdx.x; r < total; r = paged_next(r, (int)gridDim.x)) {
+        const Piece a = paged_piece(p, order, r);
         float q[kPlainHeads][8], acc[kPlainHeads][8], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
         for (int h = 0; h < kPlainHeads; ++h) {
@@ -71,63 +71,59 @@ __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const Pag
                 num += g * src[f];
                 den += g * src[p.dim + 1];
             }
-            if (a.parts == 1) paged_put<T>(p, a.b, a.head0 + h, f, den == 0.f ? 0.f : num / den);
-            else {
-                float* dst = p.partial + (((long long)a.pair * p.most + a.part) * p.chunk + h) * stride;
-                dst[f] = num;
-                if (f == 0) { dst[p.dim] = top; dst[p.dim + 1] = den; }
-            }
+            p.partial[paged_place(p, a, h) * p.dim + f] = num;
+            if (f == 0) p.stats[paged_place(p, a, h)] = make_float2(top, den);
         }
         __syncthreads();
     }
 }
 
-// The parts of a (sequence, head) joined, a warp for every eighth part; a sequence that sees nothing gets zeros.
+// The parts of a (sequence, head) joined, 32 * EACH columns by a block, a warp for every eighth part; a sequence that sees nothing gets zeros.
 constexpr int kJoinWarps = 8;
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int blocks) {
+template <typename T, int EACH>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int workers) {
     chain_enter();
-    __shared__ float state[kJoinWarps][256 + 2];
-    const int head = blockIdx.x, b = blockIdx.y, each = p.kv_heads * p.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int parts = paged_parts(paged_span(p, b).seen, p.unit, (long long)p.batch * each, blocks);
-    if (parts == 1) return;
-    const int kvh = head / p.group, in = head - kvh * p.group, stride = p.dim + 2;
-    const long long pair = (long long)b * each + kvh * p.chunks + in / p.chunk, step = (long long)p.chunk * stride;
-    const float* src = p.partial + (pair * p.most * p.chunk + in % p.chunk) * stride;
-    float top = -INFINITY, den = 0.f, num[8] = {};
+    __shared__ float state[kJoinWarps][EACH * 32 + 2];
+    const int head = blockIdx.x, b = blockIdx.y, column = blockIdx.z * EACH * 32, each = p.kv_heads * p.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int parts = paged_parts(paged_span(p, b).seen, p.unit, p.batch * each, workers);
+    const int kvh = head / p.group, in = head - kvh * p.group;
+    const long long place = ((long long)b * each + kvh * p.chunks + in / p.chunk) * p.most * p.chunk + in % p.chunk;
+    const float* src = p.partial + place * p.dim + column + lane;
+    float top = -INFINITY, den = 0.f, num[EACH] = {};
     for (int base = warp; base < parts; base += 32 * kJoinWarps) {
         const int mine = base + lane * kJoinWarps;                     // a lane's part
-        const float m = mine < parts ? src[mine * step + p.dim] : -INFINITY, l = mine < parts ? src[mine * step + p.dim + 1] : 0.f;
-        const float now = fmaxf(top, warp_max(m)), shift = now == -INFINITY ? 0.f : now, fix = exp2f(top - shift), w = l == 0.f ? 0.f : exp2f(m - shift);
+        const float2 of = mine < parts ? p.stats[place + (long long)mine * p.chunk] : make_float2(-INFINITY, 0.f);
+        const float now = fmaxf(top, warp_max(of.x)), shift = now == -INFINITY ? 0.f : now;
+        const float fix = exp2f(top - shift), w = of.y == 0.f ? 0.f : exp2f(of.x - shift);
         top = now;
-        den = den * fix + warp_sum(w * l);
+        den = den * fix + warp_sum(w * of.y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) num[j] *= fix;
+        for (int j = 0; j < EACH; ++j) num[j] *= fix;
         const int count = min(32, (parts - base + kJoinWarps - 1) / kJoinWarps);
-#pragma unroll 4
+#pragma unroll (EACH > 2 ? 2 : 8)
         for (int i = 0; i < count; ++i) {
             const float each_w = __shfl_sync(0xffffffffu, w, i);
-            const float* row = src + (base + i * kJoinWarps) * step;
+            const float* row = src + (long long)(base + i * kJoinWarps) * p.chunk * p.dim;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j * 32 + lane < p.dim) num[j] += each_w * row[j * 32 + lane];
+            for (int j = 0; j < EACH; ++j)
+                if (column + j * 32 + lane < p.dim) num[j] += each_w * row[j * 32];
         }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) state[warp][j * 32 + lane] = num[j];
-    if (lane == 0) { state[warp][256] = top; state[warp][257] = den; }
+    for (int j = 0; j < EACH; ++j) state[warp][j * 32 + lane] = num[j];
+    if (lane == 0) { state[warp][EACH * 32] = top; state[warp][EACH * 32 + 1] = den; }
     __syncthreads();
-    if (tid >= p.dim) return;
+    if (tid >= EACH * 32 || column + tid >= p.dim) return;
     float all = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, state[w][256]);
+    for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, state[w][EACH * 32]);
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) {
-        const float g = state[w][257] == 0.f ? 0.f : exp2f(state[w][256] - all);
-        sum += g * state[w][257];
+        const float g = state[w][EACH * 32 + 1] == 0.f ? 0.f : exp2f(state[w][EACH * 32] - all);
+        sum += g * state[w][EACH * 32 + 1];
         v += g * state[w][tid];
     }
-    paged_put<T>(p, b, head, tid, sum == 0.f ? 0.f : v / sum);
+    paged_put<T>(p, b, head, column + tid, sum == 0.f ? 0.f : v / sum);
 }
 
 int paged_blocks() {
@@ -140,7 +136,9 @@ int chunk_of(int group, bool fp32) {
     const int most = fp32 || group <= 8 ? 8 : 16;
     return group < most ? group : most;
 }
-int unit_of(int dim, bool fp32) { return fp32 ? 32 : dim <= 64 ? 256 : dim <= 128 ? 128 : 64; }         // a tile for each warp
+int unit_of(bool fp32) { return fp32 ? 32 : 16; }
+// Who takes a part: a block, or a warp.
+int workers_of(int dim, bool fp32) { return paged_blocks() * (fp32 ? 1 : dim <= 64 ? 16 : dim <= 128 ? 8 : 4); }
 
 template <int D, int NT>
 int mma_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
@@ -153,16 +151,22 @@ int plain_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
     if (cudaFuncSetAttribute(paged_plain_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
     return qd_launch(paged_plain_kernel<float>, dim3(blocks), dim3(kPlainWarps * 32), smem, stream, 3, p);
 }
+// Few rows: 64 columns a block, so that many blocks share the reads.
+template <typename T>
+int join_launch(const PagedParams& p, int blocks, int workers, cudaStream_t stream) {
+    if (p.heads * p.batch < 2 * blocks)
+        return qd_launch(paged_join_kernel<T, 2>, dim3(p.heads, p.batch, (p.dim + 63) / 64), dim3(kJoinWarps * 32), 0, stream, 3, p, workers);
+    return qd_launch(paged_join_kernel<T, 8>, dim3(p.heads, p.batch), dim3(kJoinWarps * 32), 0, stream, 3, p, workers);
+}
 int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
-    const int blocks = paged_blocks();
+    const int blocks = paged_blocks(), workers = workers_of(p.dim, fp32);
     const bool two = p.chunk > 8;
     int code = fp32 ? plain_launch(p, blocks, stream)
              : p.dim <= 64 ? (two ? mma_launch<64, 2>(p, blocks, stream) : mma_launch<64, 1>(p, blocks, stream))
              : p.dim <= 128 ? (two ? mma_launch<128, 2>(p, blocks, stream) : mma_launch<128, 1>(p, blocks, stream))
                             : (two ? mma_launch<256, 2>(p, blocks, stream) : mma_launch<256, 1>(p, blocks, stream));
     if (code != QD_OK) return code;
-    const dim3 grid(p.heads, p.batch), block(kJoinWarps * 32);
-    return fp32 ? qd_launch(paged_join_kernel<float>, grid, block, 0, stream, 3, p, blocks) : qd_launch(paged_join_kernel<bf16>, grid, block, 0, stream, 3, p, blocks);
+    return fp32 ? join_launch<float>(p, blocks, workers, stream) : join_launch<bf16>(p, blocks, workers, stream);
 }
 
 }  // namespace
@@ -172,12 +176,13 @@ using namespace qd;
 
 extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim) {
     if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
-    const int group = heads / kv_heads, blocks = paged_blocks();
+    const int group = heads / kv_heads;
     long long most = 0;
     for (int fp32 = 0; fp32 < 2; ++fp32)
         for (const int some : {batch < kPagedSeqs ? batch : kPagedSeqs, batch % kPagedSeqs}) {          // whole launches and the last one
+            if (!some) continue;
             const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
-            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_most(pairs, blocks) * chunk * (dim + 2);
+            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_most(pairs, workers_of(dim, fp32)) * chunk * (dim + 2);
             if (floats > most) most = floats;
         }
     return most;
@@ -199,13 +204,15 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     const bool all = (long long)window + sinks >= (long long)width * page;      // (their sum fits 32 bits otherwise)
     p.window = all ? 0 : window; p.sinks = all ? 0 : sinks;
     p.group = heads / kv_heads; p.chunk = chunk_of(p.group, is_fp32); p.chunks = (p.group + p.chunk - 1) / p.chunk;
-    p.unit = unit_of(dim, is_fp32); p.scale = scale * 1.4426950408889634f;
+    p.unit = unit_of(is_fp32); p.scale = scale * 1.4426950408889634f;
     const int size = is_fp32 ? 4 : 2;
     p.q_whole = !(((uintptr_t)q | (uintptr_t)(q_row * size) | (uintptr_t)(q_head * size)) & 15u);
-    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(page_stride * size) | (uintptr_t)(row_stride * size) | (uintptr_t)(head_stride * size)) & 15u) return QD_ERR_UNSUPPORTED;
+    if (((uintptr_t)partial | (uintptr_t)k | (uintptr_t)v | (uintptr_t)(page_stride * size) | (uintptr_t)(row_stride * size) | (uintptr_t)(head_stride * size)) & 15u) return QD_ERR_UNSUPPORTED;
     for (int b = 0; b < batch; b += kPagedSeqs) {                 // (the scratch is used again in stream order)
         p.batch = batch - b < kPagedSeqs ? batch - b : kPagedSeqs;
-        p.most = paged_most((long long)p.batch * kv_heads * p.chunks, paged_blocks());
+        const long long pairs = (long long)p.batch * kv_heads * p.chunks;
+        p.most = paged_most(pairs, workers_of(dim, is_fp32));
+        p.stats = (float2*)(p.partial + pairs * p.most * p.chunk * dim);
         p.q = (const char*)q + b * q_row * size;
         p.gate = gate ? (const char*)gate + b * gate_row * size : nullptr;
         p.out = (char*)out + (long long)b * heads * dim * size;
