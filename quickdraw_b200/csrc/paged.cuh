@@ -4,6 +4,43 @@
 
 namespace qd {
 
+// A sequence is cut into parts by its own length, the number of (sequence, key/value head, chunk of heads) triples and that of workers alone, so that
+// its result does not depend on its neighbours: as if all of the batch were as long, so that they fill some rounds of workers in least time (a part
+// costs `kPagedFixed` units beside its own: its state is written, read and joined); of cuts that are within 1 / 16 of it the finest, because beside
+// other lengths smaller parts are shared out more evenly.
+constexpr int kPagedCuts = 6, kPagedLeast = 1;
+constexpr float kPagedFixed = 1.f;
+struct PagedCuts { float each[kPagedCuts], rounds[kPagedCuts]; int most; };     // parts of a sequence (their reciprocal), rounds of workers
+static inline PagedCuts paged_cuts(long long pairs, int workers) {
+    constexpr int kRounds[kPagedCuts] = {1, 2, 3, 4, 6, 8};
+    PagedCuts c{};
+    c.most = 1;
+    for (int i = 0; i < kPagedCuts; ++i) {
+        long long parts = (long long)kRounds[i] * workers / pairs;
+        if (parts < 1) parts = 1;
+        c.each[i] = 1.f / (float)parts;
+        c.rounds[i] = (float)((pairs * parts + workers - 1) / workers);
+        c.most = (int)parts + 1;                                                  // (one more than the rounding of `each` may make of it)
+    }
+    return c;
+}
+static __device__ __forceinline__ int paged_parts(const PagedCuts& c, int seen, int unit) {
+    if (seen <= 0) return 0;
+    const int n = (seen - 1) / unit + 1;
+    float per[kPagedCuts], cost[kPagedCuts], least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPagedCuts; ++i) {
+        per[i] = fmaxf(ceilf((float)n * c.each[i]), (float)kPagedLeast);
+        cost[i] = c.rounds[i] * (per[i] + kPagedFixed);
+        least = fminf(least, cost[i]);
+    }
+    int best = n;
+#pragma unroll
+    for (int i = 0; i < kPagedCuts; ++i)
+        if (cost[i] <= least * 1.0625f) best = (int)per[i];
+    return (n + best - 1) / best;
+}
+
 struct PagedParams {
     const void* q; const void* gate; const void* k; const void* v;
     long long q_row, q_head, gate_row, gate_head, page_stride, row_stride, head_stride, table_stride;   // in elements
@@ -12,7 +49,8 @@ struct PagedParams {
     float* partial; float2* stats;      // [pair][most][heads of a chunk][dim]: weighted values; [pair][most][heads of a chunk]: maximum, sum
     int batch, heads, kv_heads, dim, pages, page, width, window, sinks;
     int group, chunk, chunks;           // query heads of a key/value head; of them at a time; how often
-    int unit, most;                     // positions of a unit; parts of a pair, at most
+    int unit;                           // positions of a unit
+    PagedCuts cuts;
     int q_whole;                        // queries in 16-byte pieces
     float scale;                        // of the scores, times log2(e)
 };
@@ -27,117 +65,82 @@ QD_DEVINL Span paged_span(const PagedParams& p, int b) {
 }
 QD_DEVINL int paged_position(const PagedParams& p, int i, int skip) { return i < p.sinks ? i : i + skip; }
 
-// A sequence is cut into parts by its own length, the number of (sequence, key/value head, chunk of heads) triples and that of workers alone, so that
-// its result does not depend on its neighbours: as if all of the batch were as long, each worker gets one part, or, if that is a long one, several
-// equal ones, because beside other lengths smaller parts are shared out more evenly.
-constexpr int kPagedLeast = 4, kPagedRound = 8, kPagedRounds = 4;
-static __host__ __device__ __forceinline__ int paged_most(long long pairs, int workers) {
-    const long long most = (long long)kPagedRounds * workers / pairs;
-    return most < 1 ? 1 : (int)most;
-}
-static __host__ __device__ __forceinline__ int paged_parts(int seen, int unit, int pairs, int workers) {
-    if (seen <= 0) return 0;
-    const int n = (seen - 1) / unit + 1;
-    const float share = (float)n * (float)pairs / (float)workers;                 // units of a worker, if all were as long
-    const int rounds = share < 2.f * kPagedRound ? 1 : share < (float)kPagedRounds * kPagedRound ? (int)(share / kPagedRound) : kPagedRounds;
-    const int parts = rounds * workers / pairs;                                   // (at most kPagedRounds * workers)
-    int per = parts > 1 ? (n + parts - 1) / parts : n;
-    if (per < kPagedLeast) per = kPagedLeast;
-    return (n + per - 1) / per;
-}
-
 template <typename T> QD_DEVINL float paged_load(const T* p) { return (float)*p; }
 template <> QD_DEVINL float paged_load<bf16>(const bf16* p) { return __bfloat162float(*p); }
 template <typename T> QD_DEVINL void paged_store(T* p, float v);
 template <> QD_DEVINL void paged_store<float>(float* p, float v) { *p = v; }
 template <> QD_DEVINL void paged_store<bf16>(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-constexpr int kPagedSeqs = 256;        // sequences of a launch
+constexpr int kPagedSeqs = 192;        // sequences of a launch
 
-// The parts of all sequences, those of the largest parts first.
-struct PagedOrder {
-    int before[kPagedSeqs + 1];         // pieces (a part of a pair each) in front of the i-th sequence's
-    int seen[kPagedSeqs];               // rows that it sees
-    uint8_t sequence[kPagedSeqs];
-};
+// Pieces (a part of a pair each) in front of each sequence's, and the rows that it sees.
+struct PagedOrder { int before[kPagedSeqs + 1], seen[kPagedSeqs]; };
 template <int THREADS>
-QD_DEVINL int paged_schedule(const PagedParams& p, PagedOrder& o, int workers) {
+QD_DEVINL int paged_schedule(const PagedParams& p, PagedOrder& o) {
     __shared__ int sums[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = p.kv_heads * p.chunks;
-    // units of a part (in `before`, for a moment), and how many sequences have larger ones
-    for (int b = tid; b < p.batch; b += THREADS) {
-        const int n = paged_span(p, b).seen, parts = paged_parts(n, p.unit, p.batch * each, workers);
-        o.before[b] = parts ? ((n - 1) / p.unit + parts) / parts : 0;
-    }
-    __syncthreads();
-    constexpr int kEach = (kPagedSeqs + THREADS - 1) / THREADS;
-    int rank[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int b = j * THREADS + tid, per = b < p.batch ? o.before[b] : 0;
-        rank[j] = 0;
-        if (b < p.batch)
-            for (int z = 0; z < p.batch; ++z) rank[j] += o.before[z] > per || (o.before[z] == per && z < b);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int b = j * THREADS + tid;
-        if (b < p.batch) { o.sequence[rank[j]] = (uint8_t)b; o.seen[rank[j]] = paged_span(p, b).seen; }
-    }
-    __syncthreads();
     int total = 0;
     for (int base = 0; base < p.batch; base += THREADS) {
-        const int i = base + tid;
-        int sum = i < p.batch ? each * paged_parts(o.seen[i], p.unit, p.batch * each, workers) : 0;
+        const int b = base + tid;
+        int sum = 0;
+        if (b < p.batch) {
+            const int seen = paged_span(p, b).seen;
+            o.seen[b] = seen;
+            sum = each * paged_parts(p.cuts, seen, p.unit);
+        }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, sum, d);
             if (lane >= d) sum += up;
         }
-        if (lane == 31) sums[warp] = sum;
-        __syncthreads();
-        int all = 0;
-        for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) sum += sums[w]; all += sums[w]; }
-        if (i < p.batch) o.before[i + 1] = total + sum;
-        total += all;
-        __syncthreads();
+        if (p.batch > 32) {
+            if (lane == 31) sums[warp] = sum;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; ++w) { const int of = sums[w]; if (w < warp) sum += of; all += of; }
+            if (b < p.batch) o.before[b + 1] = total + sum;
+            total += all;
+            __syncthreads();
+        } else if (b < p.batch) o.before[b + 1] = sum;                  // (one warp's)
     }
     if (tid == 0) o.before[0] = 0;
     __syncthreads();
-    return total;
-}
-// Rounds of pieces, one a worker, to and fro, so that who had a larger one takes a smaller one next: the piece after piece r.
-QD_DEVINL int paged_next(int r, int workers) {
-    const int round = r / workers;
-    return 2 * (round + 1) * workers - 1 - r;
+    return o.before[p.batch];
 }
 
-struct Piece { int b, kvh, head0, heads, t0, t1, skip, part, parts, pair; };
-QD_DEVINL Piece paged_piece(const PagedParams& p, const PagedOrder& o, int r) {
-    int lo = 0;
+// a / b of numbers below 2^24
+QD_DEVINL int paged_quotient(int a, int b) {
+    int q = (int)__fdividef((float)a, (float)b);
+    const int rest = a - q * b;
+    q += rest >= b ? 1 : 0;
+    return rest < 0 ? q - 1 : q;
+}
+struct Piece { int b, kvh, head0, heads, t0, t1, skip, part, pair; };
+// Piece r, of no sequence in front of `from`.
+QD_DEVINL Piece paged_piece(const PagedParams& p, const PagedOrder& o, int r, int from) {
+    int lo = from;
     for (int hi = p.batch; hi - lo > 1;) {
         const int mid = (lo + hi) >> 1;
         if (o.before[mid] <= r) lo = mid; else hi = mid;
     }
     Piece a;
-    const int each = p.kv_heads * p.chunks, n = o.seen[lo], at = r - o.before[lo];
-    a.b = o.sequence[lo];
-    a.parts = (o.before[lo + 1] - o.before[lo]) / each;
-    const int pair = at / a.parts, per = ((n + p.unit - 1) / p.unit + a.parts - 1) / a.parts * p.unit;
-    a.part = at - pair * a.parts;
-    a.kvh = pair / p.chunks;
+    const int each = p.kv_heads * p.chunks, n = o.seen[lo], at = r - o.before[lo], parts = paged_quotient(o.before[lo + 1] - o.before[lo], each);
+    const int pair = paged_quotient(at, parts), per = ((n - 1) / p.unit + parts) / parts * p.unit;
+    a.b = lo;
+    a.part = at - pair * parts;
+    a.kvh = p.chunks == 1 ? pair : paged_quotient(pair, p.chunks);
     const int chunk = pair - a.kvh * p.chunks;
     a.head0 = a.kvh * p.group + chunk * p.chunk;
     a.heads = min(p.chunk, p.group - chunk * p.chunk);
-    a.pair = a.b * each + pair;
+    a.pair = lo * each + pair;
     a.t0 = a.part * per;
     a.t1 = min(n, a.t0 + per);
-    a.skip = p.window > 0 && n == p.window + p.sinks ? min(max(__ldcg(p.lengths + a.b), 0), p.width * p.page) - n : 0;
+    a.skip = p.window > 0 && n == p.window + p.sinks ? min(max(__ldcg(p.lengths + lo), 0), p.width * p.page) - n : 0;
     return a;
 }
 
-QD_DEVINL long long paged_place(const PagedParams& p, const Piece& a, int h) { return ((long long)a.pair * p.most + a.part) * p.chunk + h; }
+QD_DEVINL long long paged_place(const PagedParams& p, const Piece& a, int h) { return ((long long)a.pair * p.cuts.most + a.part) * p.chunk + h; }
 
 template <typename T>
 QD_DEVINL void paged_put(const PagedParams& p, int b, int head, int f, float v) {

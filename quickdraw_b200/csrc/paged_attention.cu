@@ -14,9 +14,9 @@ __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const Pag
     extern __shared__ __align__(16) float plain_smem[];                // [warps][heads][dim + 2]
     __shared__ PagedOrder order;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = p.dim + 2;
-    const int total = paged_schedule<kPlainWarps * 32>(p, order, (int)gridDim.x);
-    for (int r = blockIdx.x; r < total; r = paged_next(r, (int)gridDim.x)) {
-        const Piece a = paged_piece(p, order, r);
+    const int total = paged_schedule<kPlainWarps * 32>(p, order);
+    for (int r = blockIdx.x; r < total; r += (int)gridDim.x) {
+        const Piece a = paged_piece(p, order, r, 0);
         float q[kPlainHeads][8], acc[kPlainHeads][8], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
         for (int h = 0; h < kPlainHeads; ++h) {
@@ -78,52 +78,65 @@ __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const Pag
     }
 }
 
-// The parts of a (sequence, head) joined, 32 * EACH columns by a block, a warp for every eighth part; a sequence that sees nothing gets zeros.
+// The parts of a (sequence, head) joined, 32 * EACH columns by WARPS warps that take every WARPS-th part; a sequence that sees nothing gets zeros.
 constexpr int kJoinWarps = 8;
-template <typename T, int EACH>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int workers) {
+template <typename T, int EACH, int WARPS>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p) {
     chain_enter();
-    __shared__ float state[kJoinWarps][EACH * 32 + 2];
-    const int head = blockIdx.x, b = blockIdx.y, column = blockIdx.z * EACH * 32, each = p.kv_heads * p.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int parts = paged_parts(paged_span(p, b).seen, p.unit, p.batch * each, workers);
-    const int kvh = head / p.group, in = head - kvh * p.group;
-    const long long place = ((long long)b * each + kvh * p.chunks + in / p.chunk) * p.most * p.chunk + in % p.chunk;
-    const float* src = p.partial + place * p.dim + column + lane;
+    __shared__ float state[WARPS][EACH * 32 + 2];
+    const int tid = threadIdx.x, warp = WARPS == 1 ? 0 : tid >> 5, lane = tid & 31, each = p.kv_heads * p.chunks, column = blockIdx.y * EACH * 32 + lane;
+    const int row = WARPS == 1 ? (int)blockIdx.x * kJoinWarps + (tid >> 5) : (int)blockIdx.x;
+    if (row >= p.batch * p.heads) return;
+    const int b = row / p.heads, head = row - b * p.heads, kvh = head / p.group, in = head - kvh * p.group;
+    const long long place = ((long long)b * each + kvh * p.chunks + in / p.chunk) * p.cuts.most * p.chunk + in % p.chunk;
+    const float* src = p.partial + place * p.dim + column;
+    // (read while the length is on its way; what lies behind the last part is not used)
+    int mine = warp + lane * WARPS;                                    // a lane's part
+    float2 of = mine < p.cuts.most ? p.stats[place + (long long)mine * p.chunk] : make_float2(0.f, 0.f);
+    const int parts = paged_parts(p.cuts, paged_span(p, b).seen, p.unit);
     float top = -INFINITY, den = 0.f, num[EACH] = {};
-    for (int base = warp; base < parts; base += 32 * kJoinWarps) {
-        const int mine = base + lane * kJoinWarps;                     // a lane's part
-        const float2 of = mine < parts ? p.stats[place + (long long)mine * p.chunk] : make_float2(-INFINITY, 0.f);
+    for (int base = warp; base < parts; base += 32 * WARPS) {
+        if (base != warp) of = mine < parts ? p.stats[place + (long long)mine * p.chunk] : of;
+        if (mine >= parts) of = make_float2(-INFINITY, 0.f);
         const float now = fmaxf(top, warp_max(of.x)), shift = now == -INFINITY ? 0.f : now;
         const float fix = exp2f(top - shift), w = of.y == 0.f ? 0.f : exp2f(of.x - shift);
         top = now;
         den = den * fix + warp_sum(w * of.y);
 #pragma unroll
         for (int j = 0; j < EACH; ++j) num[j] *= fix;
-        const int count = min(32, (parts - base + kJoinWarps - 1) / kJoinWarps);
-#pragma unroll (EACH > 2 ? 2 : 8)
+        const int count = min(32, (parts - base + WARPS - 1) / WARPS);
+#pragma unroll (EACH > 2 ? 2 : 16)
         for (int i = 0; i < count; ++i) {
             const float each_w = __shfl_sync(0xffffffffu, w, i);
-            const float* row = src + (long long)(base + i * kJoinWarps) * p.chunk * p.dim;
+            const float* from = src + (long long)(base + i * WARPS) * p.chunk * p.dim;
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
-                if (column + j * 32 + lane < p.dim) num[j] += each_w * row[j * 32];
+                if (column + j * 32 < p.dim) num[j] += each_w * from[j * 32];
         }
+        mine += 32 * WARPS;
     }
+    if constexpr (WARPS == 1) {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            if (column + j * 32 < p.dim) paged_put<T>(p, b, head, column + j * 32, den == 0.f ? 0.f : num[j] / den);
+    } else {
 #pragma unroll
     for (int j = 0; j < EACH; ++j) state[warp][j * 32 + lane] = num[j];
     if (lane == 0) { state[warp][EACH * 32] = top; state[warp][EACH * 32 + 1] = den; }
     __syncthreads();
-    if (tid >= EACH * 32 || column + tid >= p.dim) return;
+    const int f = blockIdx.y * EACH * 32 + tid;
+    if (tid >= EACH * 32 || f >= p.dim) return;
     float all = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, state[w][EACH * 32]);
+    for (int w = 0; w < WARPS; ++w) all = fmaxf(all, state[w][EACH * 32]);
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         const float g = state[w][EACH * 32 + 1] == 0.f ? 0.f : exp2f(state[w][EACH * 32] - all);
         sum += g * state[w][EACH * 32 + 1];
         v += g * state[w][tid];
     }
-    paged_put<T>(p, b, head, column + tid, sum == 0.f ? 0.f : v / sum);
+    paged_put<T>(p, b, head, f, sum == 0.f ? 0.f : v / sum);
+    }
 }
 
 int paged_blocks() {
@@ -136,9 +149,11 @@ int chunk_of(int group, bool fp32) {
     const int most = fp32 || group <= 8 ? 8 : 16;
     return group < most ? group : most;
 }
-int unit_of(bool fp32) { return fp32 ? 32 : 16; }
-// Who takes a part: a block, or a warp.
-int workers_of(int dim, bool fp32) { return paged_blocks() * (fp32 ? 1 : dim <= 64 ? 16 : dim <= 128 ? 8 : 4); }
+int unit_of(bool fp32) { return fp32 ? 32 : kPagedGroup * 16; }
+// Who takes a part: a block, or a group of warps.
+int workers_of(int dim, bool fp32) {
+    return paged_blocks() * (fp32 ? 1 : dim <= 64 ? PagedMma<64, 1>::kGroups : dim <= 128 ? PagedMma<128, 1>::kGroups : PagedMma<256, 1>::kGroups);
+}
 
 template <int D, int NT>
 int mma_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
@@ -151,22 +166,23 @@ int plain_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
     if (cudaFuncSetAttribute(paged_plain_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
     return qd_launch(paged_plain_kernel<float>, dim3(blocks), dim3(kPlainWarps * 32), smem, stream, 3, p);
 }
-// Few rows: 64 columns a block, so that many blocks share the reads.
+// By the number of rows: 32 columns of a row a block, a row a block, a row a warp.
 template <typename T>
-int join_launch(const PagedParams& p, int blocks, int workers, cudaStream_t stream) {
-    if (p.heads * p.batch < 2 * blocks)
-        return qd_launch(paged_join_kernel<T, 2>, dim3(p.heads, p.batch, (p.dim + 63) / 64), dim3(kJoinWarps * 32), 0, stream, 3, p, workers);
-    return qd_launch(paged_join_kernel<T, 8>, dim3(p.heads, p.batch), dim3(kJoinWarps * 32), 0, stream, 3, p, workers);
+int join_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
+    const int rows = p.heads * p.batch;
+    if (2 * rows <= blocks) return qd_launch(paged_join_kernel<T, 1, kJoinWarps>, dim3(rows, (p.dim + 31) / 32), dim3(kJoinWarps * 32), 0, stream, 3, p);
+    if (rows <= 4 * blocks) return qd_launch(paged_join_kernel<T, 8, kJoinWarps>, dim3(rows), dim3(kJoinWarps * 32), 0, stream, 3, p);
+    return qd_launch(paged_join_kernel<T, 8, 1>, dim3((rows + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, stream, 3, p);
 }
 int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
-    const int blocks = paged_blocks(), workers = workers_of(p.dim, fp32);
+    const int blocks = paged_blocks();
     const bool two = p.chunk > 8;
     int code = fp32 ? plain_launch(p, blocks, stream)
              : p.dim <= 64 ? (two ? mma_launch<64, 2>(p, blocks, stream) : mma_launch<64, 1>(p, blocks, stream))
              : p.dim <= 128 ? (two ? mma_launch<128, 2>(p, blocks, stream) : mma_launch<128, 1>(p, blocks, stream))
                             : (two ? mma_launch<256, 2>(p, blocks, stream) : mma_launch<256, 1>(p, blocks, stream));
     if (code != QD_OK) return code;
-    return fp32 ? join_launch<float>(p, blocks, workers, stream) : join_launch<bf16>(p, blocks, workers, stream);
+    return fp32 ? join_launch<float>(p, blocks, stream) : join_launch<bf16>(p, blocks, stream);
 }
 
 }  // namespace
@@ -182,7 +198,7 @@ extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_head
         for (const int some : {batch < kPagedSeqs ? batch : kPagedSeqs, batch % kPagedSeqs}) {          // whole launches and the last one
             if (!some) continue;
             const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
-            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_most(pairs, workers_of(dim, fp32)) * chunk * (dim + 2);
+            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, workers_of(dim, fp32)).most * chunk * (dim + 2);
             if (floats > most) most = floats;
         }
     return most;
@@ -211,8 +227,8 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     for (int b = 0; b < batch; b += kPagedSeqs) {                 // (the scratch is used again in stream order)
         p.batch = batch - b < kPagedSeqs ? batch - b : kPagedSeqs;
         const long long pairs = (long long)p.batch * kv_heads * p.chunks;
-        p.most = paged_most(pairs, workers_of(dim, is_fp32));
-        p.stats = (float2*)(p.partial + pairs * p.most * p.chunk * dim);
+        p.cuts = paged_cuts(pairs, workers_of(dim, is_fp32));
+        p.stats = (float2*)(p.partial + pairs * p.cuts.most * p.chunk * dim);
         p.q = (const char*)q + b * q_row * size;
         p.gate = gate ? (const char*)gate + b * gate_row * size : nullptr;
         p.out = (char*)out + (long long)b * heads * dim * size;
