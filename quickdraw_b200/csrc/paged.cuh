@@ -71,43 +71,74 @@ template <typename T> QD_DEVINL void paged_store(T* p, float v);
 template <> QD_DEVINL void paged_store<float>(float* p, float v) { *p = v; }
 template <> QD_DEVINL void paged_store<bf16>(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-constexpr int kPagedSeqs = 192;        // sequences of a launch
 
-// Pieces (a part of a pair each) in front of each sequence's, and the rows that it sees.
-struct PagedOrder { int before[kPagedSeqs + 1], seen[kPagedSeqs]; };
-template <int THREADS>
-QD_DEVINL int paged_schedule(const PagedParams& p, PagedOrder& o) {
+// Pieces (a part of a pair each) in front of each sequence's, and the rows that it sees.  Where there is more than a piece for each worker and not too
+// many sequences, those of the largest parts are first.
+constexpr int kPagedSorted = 128;
+template <int N> struct PagedOrder {
+    int before[N + 1], seen[N], sorted;
+    uint8_t sequence[kPagedSorted];
+};
+template <int N, int THREADS>
+QD_DEVINL int paged_schedule(const PagedParams& p, PagedOrder<N>& o, int workers) {
     __shared__ int sums[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = p.kv_heads * p.chunks;
-    int total = 0;
-    for (int base = 0; base < p.batch; base += THREADS) {
-        const int b = base + tid;
-        int sum = 0;
-        if (b < p.batch) {
-            const int seen = paged_span(p, b).seen;
-            o.seen[b] = seen;
-            sum = each * paged_parts(p.cuts, seen, p.unit);
-        }
+    // pieces of the i-th sequence, given by `count`, summed up in order
+    const auto sum_up = [&](const auto& count) {
+        int total = 0;
+        for (int base = 0; base < p.batch; base += THREADS) {
+            const int i = base + tid;
+            int sum = i < p.batch ? each * count(i) : 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += up;
-        }
-        if (p.batch > 32) {
-            if (lane == 31) sums[warp] = sum;
-            __syncthreads();
-            int all = 0;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += up;
+            }
+            if (p.batch > 32) {
+                if (lane == 31) sums[warp] = sum;
+                __syncthreads();
+                int all = 0;
 #pragma unroll
-            for (int w = 0; w < THREADS / 32; ++w) { const int of = sums[w]; if (w < warp) sum += of; all += of; }
-            if (b < p.batch) o.before[b + 1] = total + sum;
-            total += all;
-            __syncthreads();
-        } else if (b < p.batch) o.before[b + 1] = sum;                  // (one warp's)
-    }
-    if (tid == 0) o.before[0] = 0;
+                for (int w = 0; w < THREADS / 32; ++w) { const int of = sums[w]; if (w < warp) sum += of; all += of; }
+                if (i < p.batch) o.before[i + 1] = total + sum;
+                total += all;
+                __syncthreads();
+            } else if (i < p.batch) o.before[i + 1] = sum;              // (one warp's)
+        }
+        if (tid == 0) o.before[0] = 0;
+        __syncthreads();
+        return o.before[p.batch];
+    };
+    if (tid == 0) o.sorted = 0;
+    int mine = 0, parts = 0;
+    const int total = sum_up([&](int b) {
+        mine = paged_span(p, b).seen;
+        o.seen[b] = mine;
+        return parts = paged_parts(p.cuts, mine, p.unit);
+    });
+    if (total <= workers || p.batch > kPagedSorted || p.batch > THREADS || p.batch == 1) return total;
+    int* per = o.before;                                                // units of a part, for a moment
     __syncthreads();
-    return o.before[p.batch];
+    if (tid < kPagedSorted) per[tid] = tid < p.batch && parts ? ((mine - 1) / p.unit + parts) / parts : -1;
+    __syncthreads();
+    int rank = 0;
+    if (tid < p.batch)
+        for (int z = 0; z < p.batch; z += 4) {                          // (behind the last: -1)
+            const int4 of = *reinterpret_cast<const int4*>(per + z);
+            const int own = per[tid];
+            rank += of.x > own || (of.x == own && z < tid);
+            rank += of.y > own || (of.y == own && z + 1 < tid);
+            rank += of.z > own || (of.z == own && z + 2 < tid);
+            rank += of.w > own || (of.w == own && z + 3 < tid);
+        }
+    __syncthreads();
+    if (tid < p.batch) { o.sequence[rank] = (uint8_t)tid; o.seen[rank] = mine; }
+    if (tid == 0) o.sorted = 1;
+    __syncthreads();
+    return sum_up([&](int i) { return paged_parts(p.cuts, o.seen[i], p.unit); });
 }
+// Rounds of pieces, one a worker, to and fro, so that who had a larger one takes a smaller one next: the piece after piece r.
+QD_DEVINL int paged_next(int r, int workers) { return 2 * (r / workers + 1) * workers - 1 - r; }
 
 // a / b of numbers below 2^24
 QD_DEVINL int paged_quotient(int a, int b) {
@@ -116,9 +147,10 @@ QD_DEVINL int paged_quotient(int a, int b) {
     q += rest >= b ? 1 : 0;
     return rest < 0 ? q - 1 : q;
 }
-struct Piece { int b, kvh, head0, heads, t0, t1, skip, part, pair; };
-// Piece r, of no sequence in front of `from`.
-QD_DEVINL Piece paged_piece(const PagedParams& p, const PagedOrder& o, int r, int from) {
+struct Piece { int at, b, kvh, head0, heads, t0, t1, skip, part, pair; };
+// Piece r, of no sequence in front of the `from`-th.
+template <int N>
+QD_DEVINL Piece paged_piece(const PagedParams& p, const PagedOrder<N>& o, int r, int from) {
     int lo = from;
     for (int hi = p.batch; hi - lo > 1;) {
         const int mid = (lo + hi) >> 1;
@@ -127,16 +159,17 @@ QD_DEVINL Piece paged_piece(const PagedParams& p, const PagedOrder& o, int r, in
     Piece a;
     const int each = p.kv_heads * p.chunks, n = o.seen[lo], at = r - o.before[lo], parts = paged_quotient(o.before[lo + 1] - o.before[lo], each);
     const int pair = paged_quotient(at, parts), per = ((n - 1) / p.unit + parts) / parts * p.unit;
-    a.b = lo;
+    a.at = lo;
+    a.b = o.sorted ? o.sequence[lo] : lo;
     a.part = at - pair * parts;
     a.kvh = p.chunks == 1 ? pair : paged_quotient(pair, p.chunks);
     const int chunk = pair - a.kvh * p.chunks;
     a.head0 = a.kvh * p.group + chunk * p.chunk;
     a.heads = min(p.chunk, p.group - chunk * p.chunk);
-    a.pair = lo * each + pair;
+    a.pair = a.b * each + pair;
     a.t0 = a.part * per;
     a.t1 = min(n, a.t0 + per);
-    a.skip = p.window > 0 && n == p.window + p.sinks ? min(max(__ldcg(p.lengths + lo), 0), p.width * p.page) - n : 0;
+    a.skip = p.window > 0 && n == p.window + p.sinks ? min(max(__ldcg(p.lengths + a.b), 0), p.width * p.page) - n : 0;
     return a;
 }
 

@@ -7,15 +7,15 @@ namespace qd {
 namespace {
 
 // A warp per position, a lane for every 32nd feature, fp32 sums.
-constexpr int kPlainWarps = 8, kPlainHeads = 8;
+constexpr int kPlainWarps = 8, kPlainHeads = 8, kPlainSeqs = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const PagedParams p) {
     chain_enter();
     extern __shared__ __align__(16) float plain_smem[];                // [warps][heads][dim + 2]
-    __shared__ PagedOrder order;
+    __shared__ __align__(16) PagedOrder<kPlainSeqs> order;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = p.dim + 2;
-    const int total = paged_schedule<kPlainWarps * 32>(p, order);
-    for (int r = blockIdx.x; r < total; r += (int)gridDim.x) {
+    const int total = paged_schedule<kPlainSeqs, kPlainWarps * 32>(p, order, (int)gridDim.x);
+    for (int r = blockIdx.x; r < total; r = paged_next(r, (int)gridDim.x)) {
         const Piece a = paged_piece(p, order, r, 0);
         float q[kPlainHeads][8], acc[kPlainHeads][8], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
@@ -155,6 +155,9 @@ int workers_of(int dim, bool fp32) {
     return paged_blocks() * (fp32 ? 1 : dim <= 64 ? PagedMma<64, 1>::kGroups : dim <= 128 ? PagedMma<128, 1>::kGroups : PagedMma<256, 1>::kGroups);
 }
 
+// Sequences of a launch.
+int seqs_of(int dim, int chunk, bool fp32) { return fp32 ? kPlainSeqs : dim > 128 && chunk > 8 ? PagedMma<256, 2>::kSeqs : PagedMma<256, 1>::kSeqs; }
+
 template <int D, int NT>
 int mma_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
     constexpr int kSmem = PagedMma<D, NT>::kSmem;
@@ -194,13 +197,15 @@ extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_head
     if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
     const int group = heads / kv_heads;
     long long most = 0;
-    for (int fp32 = 0; fp32 < 2; ++fp32)
-        for (const int some : {batch < kPagedSeqs ? batch : kPagedSeqs, batch % kPagedSeqs}) {          // whole launches and the last one
+    for (int fp32 = 0; fp32 < 2; ++fp32) {
+        const int seqs = seqs_of(dim, chunk_of(group, fp32), fp32);
+        for (const int some : {batch < seqs ? batch : seqs, batch % seqs}) {          // whole launches and the last one
             if (!some) continue;
             const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
             const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, workers_of(dim, fp32)).most * chunk * (dim + 2);
             if (floats > most) most = floats;
         }
+    }
     return most;
 }
 
@@ -224,8 +229,9 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     const int size = is_fp32 ? 4 : 2;
     p.q_whole = !(((uintptr_t)q | (uintptr_t)(q_row * size) | (uintptr_t)(q_head * size)) & 15u);
     if (((uintptr_t)partial | (uintptr_t)k | (uintptr_t)v | (uintptr_t)(page_stride * size) | (uintptr_t)(row_stride * size) | (uintptr_t)(head_stride * size)) & 15u) return QD_ERR_UNSUPPORTED;
-    for (int b = 0; b < batch; b += kPagedSeqs) {                 // (the scratch is used again in stream order)
-        p.batch = batch - b < kPagedSeqs ? batch - b : kPagedSeqs;
+    const int seqs = seqs_of(dim, p.chunk, is_fp32);
+    for (int b = 0; b < batch; b += seqs) {                 // (the scratch is used again in stream order)
+        p.batch = batch - b < seqs ? batch - b : seqs;
         const long long pairs = (long long)p.batch * kv_heads * p.chunks;
         p.cuts = paged_cuts(pairs, workers_of(dim, is_fp32));
         p.stats = (float2*)(p.partial + pairs * p.cuts.most * p.chunk * dim);
