@@ -1,82 +1,11 @@
 // Attention of one new token of every sequence over keys and values in pages:
 //   out[b, h] = sum_p softmax_p(scale q[b, h] . k[p]) v[p],   row p of sequence b in pool[table[b][p / page]][p mod page],
 // over the positions p that the sequence sees (all, or the first few and a window), times sigmoid(gate) where given.
+#include "paged_fma.cuh"
 #include "paged_mma.cuh"
 
 namespace qd {
 namespace {
-
-// A warp per position, a lane for every 32nd feature, fp32 sums.
-constexpr int kPlainWarps = 8, kPlainHeads = 8, kPlainSeqs = 1024;
-template <typename T>
-__global__ void __launch_bounds__(kPlainWarps * 32) paged_plain_kernel(const PagedParams p) {
-    chain_enter();
-    extern __shared__ __align__(16) float plain_smem[];                // [warps][heads][dim + 2]
-    __shared__ __align__(16) PagedOrder<kPlainSeqs> order;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, stride = p.dim + 2;
-    const int total = paged_schedule<kPlainSeqs, kPlainWarps * 32>(p, order, (int)gridDim.x);
-    for (int r = blockIdx.x; r < total; r = paged_next(r, (int)gridDim.x)) {
-        const Piece a = paged_piece(p, order, r, 0);
-        float q[kPlainHeads][8], acc[kPlainHeads][8], m[kPlainHeads], l[kPlainHeads];
-#pragma unroll
-        for (int h = 0; h < kPlainHeads; ++h) {
-            m[h] = -INFINITY; l[h] = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int f = j * 32 + lane;
-                acc[h][j] = 0.f;
-                q[h][j] = h < a.heads && f < p.dim ? paged_load((const T*)p.q + a.b * p.q_row + (a.head0 + h) * p.q_head + f) : 0.f;
-            }
-        }
-        for (int i = a.t0 + warp; i < a.t1; i += kPlainWarps) {
-            const int position = paged_position(p, i, a.skip), page = p.table[a.b * p.table_stride + position / p.page];
-            if (page < 0 || page >= p.pages) continue;
-            const long long at = page * p.page_stride + position % p.page * p.row_stride + a.kvh * p.head_stride;
-            float k[8], v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int f = j * 32 + lane;
-                k[j] = f < p.dim ? paged_load((const T*)p.k + at + f) : 0.f;
-                v[j] = f < p.dim ? paged_load((const T*)p.v + at + f) : 0.f;
-            }
-#pragma unroll
-            for (int h = 0; h < kPlainHeads; ++h) {
-                float dot = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) dot += q[h][j] * k[j];
-                const float s = warp_sum(dot) * p.scale, top = fmaxf(m[h], s);
-                const float fix = m[h] == -INFINITY ? 0.f : exp2f(m[h] - top), w = s == -INFINITY ? 0.f : exp2f(s - top);
-                l[h] = l[h] * fix + w;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc[h][j] = acc[h][j] * fix + w * v[j];
-                m[h] = top;
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < kPlainHeads; ++h) {
-            float* dst = plain_smem + (warp * kPlainHeads + h) * stride;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j * 32 + lane < p.dim) dst[j * 32 + lane] = acc[h][j];
-            if (lane == 0) { dst[p.dim] = m[h]; dst[p.dim + 1] = l[h]; }
-        }
-        __syncthreads();
-        for (int i = tid; i < a.heads * p.dim; i += kPlainWarps * 32) {
-            const int h = i / p.dim, f = i % p.dim;
-            float top = -INFINITY, num = 0.f, den = 0.f;
-            for (int w = 0; w < kPlainWarps; ++w) top = fmaxf(top, plain_smem[(w * kPlainHeads + h) * stride + p.dim]);
-            for (int w = 0; w < kPlainWarps; ++w) {
-                const float* src = plain_smem + (w * kPlainHeads + h) * stride;
-                const float g = src[p.dim + 1] == 0.f ? 0.f : exp2f(src[p.dim] - top);
-                num += g * src[f];
-                den += g * src[p.dim + 1];
-            }
-            p.partial[paged_place(p, a, h) * p.dim + f] = num;
-            if (f == 0) p.stats[paged_place(p, a, h)] = make_float2(top, den);
-        }
-        __syncthreads();
-    }
-}
 
 // The parts of a (sequence, head) joined, 32 * EACH columns by WARPS warps that take every WARPS-th part; a sequence that sees nothing gets zeros.
 constexpr int kJoinWarps = 8;
@@ -144,31 +73,34 @@ int paged_blocks() {
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     return sms > 0 ? sms : 148;
 }
-// Query heads at a time: eight columns of a tensor-core instruction, or twice as many on the same keys and values.
+// Query heads at a time.
 int chunk_of(int group, bool fp32) {
     const int most = fp32 || group <= 8 ? 8 : 16;
     return group < most ? group : most;
 }
-int unit_of(bool fp32) { return fp32 ? 32 : kPagedGroup * 16; }
-// Who takes a part: a block, or a group of warps.
-int workers_of(int dim, bool fp32) {
-    return paged_blocks() * (fp32 ? 1 : dim <= 64 ? PagedMma<64, 1>::kGroups : dim <= 128 ? PagedMma<128, 1>::kGroups : PagedMma<256, 1>::kGroups);
+// The work on a tile for a head dimension, a type and a number of heads at a time: go(Work).
+template <typename Go>
+auto with_work(int dim, int chunk, bool fp32, const Go& go) {
+    if (fp32)
+        return chunk <= 4 ? dim <= 64 ? go((PagedFma<64, 4>*)nullptr) : dim <= 128 ? go((PagedFma<128, 4>*)nullptr) : go((PagedFma<256, 4>*)nullptr)
+                          : dim <= 64 ? go((PagedFma<64, 8>*)nullptr) : dim <= 128 ? go((PagedFma<128, 8>*)nullptr) : go((PagedFma<256, 8>*)nullptr);
+    return chunk <= 8 ? dim <= 64 ? go((PagedMma<64, 1>*)nullptr) : dim <= 128 ? go((PagedMma<128, 1>*)nullptr) : go((PagedMma<256, 1>*)nullptr)
+                      : dim <= 64 ? go((PagedMma<64, 2>*)nullptr) : dim <= 128 ? go((PagedMma<128, 2>*)nullptr) : go((PagedMma<256, 2>*)nullptr);
+}
+struct Plan { int seqs, workers, unit; };          // sequences of a launch, groups of warps that take parts, positions of a unit
+Plan plan_of(int dim, int chunk, bool fp32) {
+    return with_work(dim, chunk, fp32, [](auto* work) {
+        using W = std::remove_pointer_t<decltype(work)>;
+        return Plan{W::kSeqs, paged_blocks() * PagedTiles<W>::kGroups, PagedTiles<W>::kStride};
+    });
+}
+template <class W>
+int tiles_launch(const PagedParams& p, cudaStream_t stream) {
+    constexpr int kSmem = PagedTiles<W>::kSmem;
+    if (cudaFuncSetAttribute(paged_tiles_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return QD_ERR_LAUNCH;
+    return qd_launch(paged_tiles_kernel<W>, dim3(paged_blocks()), dim3(PagedTiles<W>::kThreads), kSmem, stream, 3, p);
 }
 
-// Sequences of a launch.
-int seqs_of(int dim, int chunk, bool fp32) { return fp32 ? kPlainSeqs : dim > 128 && chunk > 8 ? PagedMma<256, 2>::kSeqs : PagedMma<256, 1>::kSeqs; }
-
-template <int D, int NT>
-int mma_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
-    constexpr int kSmem = PagedMma<D, NT>::kSmem;
-    if (cudaFuncSetAttribute(paged_mma_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return QD_ERR_LAUNCH;
-    return qd_launch(paged_mma_kernel<D, NT>, dim3(blocks), dim3(PagedMma<D, NT>::kThreads), kSmem, stream, 3, p);
-}
-int plain_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
-    const size_t smem = sizeof(float) * kPlainWarps * kPlainHeads * (p.dim + 2);
-    if (cudaFuncSetAttribute(paged_plain_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
-    return qd_launch(paged_plain_kernel<float>, dim3(blocks), dim3(kPlainWarps * 32), smem, stream, 3, p);
-}
 // By the number of rows: 32 columns of a row a block, a row a block, a row a warp.
 template <typename T>
 int join_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
@@ -178,14 +110,9 @@ int join_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
     return qd_launch(paged_join_kernel<T, 8, 1>, dim3((rows + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, stream, 3, p);
 }
 int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
-    const int blocks = paged_blocks();
-    const bool two = p.chunk > 8;
-    int code = fp32 ? plain_launch(p, blocks, stream)
-             : p.dim <= 64 ? (two ? mma_launch<64, 2>(p, blocks, stream) : mma_launch<64, 1>(p, blocks, stream))
-             : p.dim <= 128 ? (two ? mma_launch<128, 2>(p, blocks, stream) : mma_launch<128, 1>(p, blocks, stream))
-                            : (two ? mma_launch<256, 2>(p, blocks, stream) : mma_launch<256, 1>(p, blocks, stream));
+    const int code = with_work(p.dim, p.chunk, fp32, [&](auto* work) { return tiles_launch<std::remove_pointer_t<decltype(work)>>(p, stream); });
     if (code != QD_OK) return code;
-    return fp32 ? join_launch<float>(p, blocks, stream) : join_launch<bf16>(p, blocks, stream);
+    return fp32 ? join_launch<float>(p, paged_blocks(), stream) : join_launch<bf16>(p, paged_blocks(), stream);
 }
 
 }  // namespace
@@ -198,11 +125,11 @@ extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_head
     const int group = heads / kv_heads;
     long long most = 0;
     for (int fp32 = 0; fp32 < 2; ++fp32) {
-        const int seqs = seqs_of(dim, chunk_of(group, fp32), fp32);
-        for (const int some : {batch < seqs ? batch : seqs, batch % seqs}) {          // whole launches and the last one
+        const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
+        const Plan plan = plan_of(dim, chunk, fp32);
+        for (const int some : {batch < plan.seqs ? batch : plan.seqs, batch % plan.seqs}) {          // whole launches and the last one
             if (!some) continue;
-            const int chunk = chunk_of(group, fp32), chunks = (group + chunk - 1) / chunk;
-            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, workers_of(dim, fp32)).most * chunk * (dim + 2);
+            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, plan.workers).most * chunk * (dim + 2);
             if (floats > most) most = floats;
         }
     }
@@ -225,15 +152,15 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     const bool all = (long long)window + sinks >= (long long)width * page;      // (their sum fits 32 bits otherwise)
     p.window = all ? 0 : window; p.sinks = all ? 0 : sinks;
     p.group = heads / kv_heads; p.chunk = chunk_of(p.group, is_fp32); p.chunks = (p.group + p.chunk - 1) / p.chunk;
-    p.unit = unit_of(is_fp32); p.scale = scale * 1.4426950408889634f;
+    const Plan plan = plan_of(dim, p.chunk, is_fp32);
+    p.unit = plan.unit; p.scale = scale * 1.4426950408889634f;
     const int size = is_fp32 ? 4 : 2;
     p.q_whole = !(((uintptr_t)q | (uintptr_t)(q_row * size) | (uintptr_t)(q_head * size)) & 15u);
     if (((uintptr_t)partial | (uintptr_t)k | (uintptr_t)v | (uintptr_t)(page_stride * size) | (uintptr_t)(row_stride * size) | (uintptr_t)(head_stride * size)) & 15u) return QD_ERR_UNSUPPORTED;
-    const int seqs = seqs_of(dim, p.chunk, is_fp32);
-    for (int b = 0; b < batch; b += seqs) {                 // (the scratch is used again in stream order)
-        p.batch = batch - b < seqs ? batch - b : seqs;
+    for (int b = 0; b < batch; b += plan.seqs) {                 // (the scratch is used again in stream order)
+        p.batch = batch - b < plan.seqs ? batch - b : plan.seqs;
         const long long pairs = (long long)p.batch * kv_heads * p.chunks;
-        p.cuts = paged_cuts(pairs, workers_of(dim, is_fp32));
+        p.cuts = paged_cuts(pairs, plan.workers);
         p.stats = (float2*)(p.partial + pairs * p.cuts.most * p.chunk * dim);
         p.q = (const char*)q + b * q_row * size;
         p.gate = gate ? (const char*)gate + b * gate_row * size : nullptr;
