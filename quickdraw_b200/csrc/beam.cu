@@ -22,15 +22,6 @@ QD_DEVINL float key_logit(unsigned long long key) {
     return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
 }
 QD_DEVINL int key_index(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
-QD_DEVINL unsigned long long warp_most(unsigned long long k) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, d);
-        k = other > k ? other : k;
-    }
-    return k;
-}
-
 template <typename T> QD_DEVINL float logit_of(T v);
 template <> QD_DEVINL float logit_of<float>(float v) { return v; }
 template <> QD_DEVINL float logit_of<bf16>(bf16 v) { return __bfloat162float(v); }
@@ -39,138 +30,282 @@ struct SelectParams {
     const void* logits; long long row_stride;                 // elements from a row to the next
     const float* scores; const uint8_t* finished;
     unsigned long long* keys;                                 // [row][split][candidates], descending; 0: none
-    float2* sums;                                             // [row][split]: maximum, sum of exp(x - maximum)
+    double2* sums;                                            // [row][split]: maximum, sum of exp(x - maximum)
     float* scores_out; int* parents_out; long long* tokens_out;
-    int batch, beams, vocab, candidates, splits, eos, placed;
+    int batch, beams, vocab, candidates, splits, eos, placed, fp32;
 };
 
-constexpr int kPartThreads = 512;
-template <typename T>
+// Descending order of 32 keys, one a lane.
+QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, d);
+            const bool upper = lane & d, ascending = lane & size;               // (of the last round: lane & 32, never)
+            key = (other > key) != (upper != ascending) ? other : key;
+        }
+    return key;
+}
+
+// A block per piece of a row, one pass: eight logits a thread at a time, their maximum and sum of exponentials, and a list of the keys above a bound that
+// `candidates` keys seen so far reach.  The bound comes from the first chunk (of each warp's 32 largest keys the candidates-th, of these the largest),
+// and again where more than a few threads have a key above it; it rises to the candidates-th of the list when that grows.
+constexpr int kPartThreads = 256, kPartEach = 8, kPartMany = 48, kPartList = 256;
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
     chain_enter();
-    __shared__ float red[kPartThreads / 32];
-    __shared__ unsigned long long best[kPartThreads / 32];
-    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    extern __shared__ __align__(16) unsigned long long part_list[];             // kPartList, and what a chunk can add: kPartMany threads' keys, or those of `candidates` lanes of each warp
+    __shared__ unsigned long long bounds[kPartThreads / 32];
+    __shared__ double2 sums[kPartThreads / 32];
+    __shared__ int count;
+    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates;
     if (p.finished && p.finished[row]) return;
     const T* x = (const T*)p.logits + row * p.row_stride;
-    const int lo = (int)((long long)p.vocab * split / p.splits), hi = (int)((long long)p.vocab * (split + 1) / p.splits);
-    float top = -INFINITY, sum = 0.f;
-    for (int i = lo + tid; i < hi; i += kPartThreads) top = fmaxf(top, logit_of(x[i]));
-    top = warp_max(top);
-    if (lane == 0) red[warp] = top;
+    const int lo = (int)((long long)(p.vocab / 8) * split / p.splits) * 8;
+    const int hi = split + 1 == p.splits ? p.vocab : (int)((long long)(p.vocab / 8) * (split + 1) / p.splits) * 8;
+    if (tid == 0) count = 0;
+    // the thread's j-th logit of the chunk from `base`: two pieces of four of fp32, one of eight of bf16, or single ones
+    constexpr int kRun = !WHOLE ? 1 : sizeof(T) == 4 ? 4 : 8;
+    const auto place = [&](int base, int j) { return base + j / kRun * (kRun * kPartThreads) + tid * kRun + j % kRun; };
+    const auto fetch = [&](int base, float (&v)[kPartEach]) {
+#pragma unroll
+        for (int j = 0; j < kPartEach; j += kRun) {
+            const int i = place(base, j);
+            if (WHOLE && i + kRun <= hi) {
+                const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + i));
+                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (sizeof(T) == 4) v[j + e] = __uint_as_float(w[e]);
+                    else { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kRun; ++e) v[j + e] = i + e < hi ? logit_of(x[i + e]) : -INFINITY;
+            }
+        }
+    };
+    // the `K` largest of the list, in order: a thread counts for its keys how many are larger
+    const auto keep = [&](unsigned long long* into, int n) {
+        for (int i = tid; i < n; i += kPartThreads) {
+            const unsigned long long key = part_list[i];
+            int rank = 0;
+            for (int z = 0; z < n; ++z) rank += part_list[z] > key;
+            if (rank < K) into[rank] = key;
+        }
+    };
+    unsigned long long* out = p.keys + ((long long)row * p.splits + split) * K;
+    float top = -INFINITY, next[kPartEach];
+    double sum = 0.0;                  // of sums of eight: 32 bits would lose a ten-millionth with every few terms
+    unsigned long long bound = 0;
+    fetch(lo, next);
     __syncthreads();
-    for (int w = 0; w < kPartThreads / 32; ++w) top = fmaxf(top, red[w]);
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += kPartThreads) {
-        const float v = logit_of(x[i]);
-        sum += v == -INFINITY ? 0.f : expf(v - top);          // (NaN and infinity go on)
+    for (int base = lo; base < hi; base += kPartThreads * kPartEach) {
+        float v[kPartEach], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kPartEach; ++j) { v[j] = next[j]; most = fmaxf(most, v[j]); }
+        if (base + kPartThreads * kPartEach < hi) fetch(base + kPartThreads * kPartEach, next);
+        if (most > top) { sum *= (double)exp2f((top - most) * 1.4426950408889634f); top = most; }
+        const float shift = top == -INFINITY ? 0.f : top;
+        float e[kPartEach];
+#pragma unroll
+        for (int j = 0; j < kPartEach; ++j) e[j] = exp2f((v[j] - shift) * 1.4426950408889634f);      // (NaN and infinity go on)
+        sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+        // the thread's largest key; places behind the end have none
+        unsigned long long mine = 0;
+        if (most >= key_logit(bound) || bound == 0) {
+#pragma unroll
+            for (int j = 0; j < kPartEach; ++j) {
+                const unsigned long long key = place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0;
+                mine = key > mine ? key : mine;
+            }
+        }
+        const int above = __syncthreads_count(mine > bound);
+        if (above == 0) continue;
+        if (above > kPartMany) {
+            const unsigned long long sorted = warp_sorted(mine, lane), kth = __shfl_sync(0xffffffffu, sorted, K - 1);
+            if (lane == 0) bounds[warp] = kth ? kth - 1 : 0;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kPartThreads / 32; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+        }
+        if (mine > bound) {
+#pragma unroll
+            for (int j = 0; j < kPartEach; ++j) {
+                const unsigned long long key = place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0;
+                if (key > bound) part_list[atomicAdd(&count, 1)] = key;
+            }
+        }
+        __syncthreads();
+        const int n = count;
+        if (n > kPartList || (base == lo && n > 2 * K && hi - lo > 4 * kPartThreads * kPartEach)) {
+            keep(out, n);                                                       // (the results' place serves as scratch)
+            __syncthreads();
+            if (tid < K) part_list[tid] = out[tid];
+            bound = out[K - 1];
+            if (tid == 0) count = K;
+            __syncthreads();
+        }
     }
-    sum = warp_sum(sum);
-    if (lane == 0) red[warp] = sum;
+    const int n = count;
+    for (int k = n + tid; k < K; k += kPartThreads) out[k] = 0;
+    keep(out, n);
+    // sums of the threads to the block's largest
+    const float warp_top = warp_max(top);
+    if (lane == 0) sums[warp].x = warp_top;
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kPartThreads / 32; ++w) all = fmaxf(all, (float)sums[w].x);
+    sum = sum == 0.0 ? 0.0 : sum * exp((double)top - (double)all);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) sums[warp].y = sum;
     __syncthreads();
     if (tid == 0) {
-        float all = 0.f;
-        for (int w = 0; w < kPartThreads / 32; ++w) all += red[w];
-        p.sums[(long long)row * p.splits + split] = make_float2(top, all);
-    }
-    unsigned long long last = ~0ull, *keys = p.keys + ((long long)row * p.splits + split) * p.candidates;
-    for (int k = 0; k < p.candidates; ++k) {
-        unsigned long long mine = 0;
-        for (int i = lo + tid; i < hi; i += kPartThreads) {
-            const unsigned long long key = logit_key(logit_of(x[i]), i);
-            if (key < last && key > mine) mine = key;
-        }
-        mine = warp_most(mine);
-        __syncthreads();
-        if (lane == 0) best[warp] = mine;
-        __syncthreads();
-        for (int w = 0; w < kPartThreads / 32; ++w) mine = best[w] > mine ? best[w] : mine;
-        last = mine;
-        if (tid == 0) keys[k] = mine;
+        double total = 0.0;
+        for (int w = 0; w < kPartThreads / 32; ++w) total += sums[w].y;
+        p.sums[(long long)row * p.splits + split] = make_double2((double)all, total);
     }
 }
 
-// A block per group: a warp joins a beam's pieces, then one warp merges the beams, a lane each.
+// A block per group: a warp joins a beam's pieces, then all beams' continuations are put in order.
 constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(kMergeWarps * 32) select_merge_kernel(const SelectParams p) {
     chain_enter();
     extern __shared__ __align__(16) unsigned char merge_smem[];
-    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates;
+    __shared__ double best[kMostBeams], partial[kMergeWarps];
+    __shared__ int order[kMostBeams];
+    __shared__ unsigned near;
+    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates, lists = p.splits < K ? p.splits : K;
     double* total = reinterpret_cast<double*>(merge_smem);                                  // [beams][K], descending
-    unsigned long long* lists = reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)warp * p.splits * K;
-    int* token = reinterpret_cast<int*>(reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)kMergeWarps * p.splits * K);   // -1: none
+    unsigned long long* list = reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)warp * lists * K;
+    int* token = reinterpret_cast<int*>(reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)kMergeWarps * lists * K);   // -1: none
     for (int i = warp; i < p.beams; i += kMergeWarps) {
         const long long row = (long long)group * p.beams + i;
         const float score = p.scores[row];
         const bool done = p.finished && p.finished[row];
+        const unsigned long long* keys = p.keys + row * p.splits * K;
+        const unsigned long long head = lane < p.splits && !done ? keys[lane * K] : 0;
         double lse = 0.0;
         bool counts = isfinite(score);
         if (!done) {
-            const float2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_float2(-INFINITY, 0.f);
-            const float top = warp_max(s.x);
+            const double2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_double2(-INFINITY, 0.0);
+            const float top = warp_max((float)s.x);
             const bool odd = __any_sync(0xffffffffu, lane < p.splits && (s.x != s.x || s.y != s.y));
-            double sum = s.y == 0.f ? 0.0 : (double)s.y * exp((double)s.x - (double)top);
+            double sum = s.y == 0.0 ? 0.0 : s.y * exp(s.x - (double)top);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             lse = (double)top + log(sum);
             counts = counts && !odd && isfinite(lse);
         }
-        if (done || !counts) {
+        for (int k = lane; k < K; k += 32) {
             // the end at no cost, and what never follows, in the order of the tokens
-            for (int k = lane; k < K; k += 32) {
-                int t = k;
-                double v = -INFINITY;
-                if (done && counts) {
-                    t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
-                    if (k == 0) v = score;
-                }
-                total[i * K + k] = v;
-                token[i * K + k] = t < p.vocab ? t : -1;
+            int t = k;
+            double v = -INFINITY;
+            if (done && counts) {
+                t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
+                if (k == 0) v = score;
             }
-            continue;
+            total[i * K + k] = v;
+            token[i * K + k] = (done || !counts) && t < p.vocab ? t : -1;
         }
-        for (int k = lane; k < p.splits * K; k += 32) lists[k] = p.keys[row * p.splits * K + k];
         __syncwarp();
-        int at = 0;
-        unsigned long long head = lane < p.splits ? lists[lane * K] : 0;
-        for (int k = 0; k < K; ++k) {
-            const unsigned long long most = warp_most(head);
-            if (lane == 0) {
-                total[i * K + k] = (double)score + ((double)key_logit(most) - lse);
-                token[i * K + k] = most ? key_index(most) : -1;
+        if (done || !counts) continue;
+        // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
+        const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
+        int n = 0;
+        for (int k = lane; k < (p.splits * K + 31) / 32 * 32; k += 32) {
+            const unsigned long long key = k < p.splits * K ? keys[k] : 0;
+            const bool in = key && key >= bound;
+            const unsigned all = __ballot_sync(0xffffffffu, in);
+            if (in) list[n + __popc(all & ((1u << lane) - 1u))] = key;
+            n += __popc(all);
+        }
+        __syncwarp();
+        for (int k = lane; k < n; k += 32) {
+            const unsigned long long key = list[k];
+            int rank = 0;
+            for (int z = 0; z < n; ++z) rank += list[z] > key;
+            if (rank < K) {
+                total[i * K + rank] = (double)score + ((double)key_logit(key) - lse);
+                token[i * K + rank] = key_index(key);
             }
-            if (most && head == most) { ++at; head = at < K ? lists[lane * K + at] : 0; }
         }
         __syncwarp();
     }
     __syncthreads();
-    if (warp) return;
-    int at = 0, parent = 0, chosen = 0;
-    double best = 0.0;
-    for (int k = 0; k < K; ++k) {
-        const bool has = lane < p.beams && at < K && token[lane * K + at] >= 0;
-        const double mine = has ? total[lane * K + at] : 0.0;
-        double v = mine;
-        int who = has ? lane : 32;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, v, d);
-            const int ow = __shfl_xor_sync(0xffffffffu, who, d);
-            if (ow < 32 && (who == 32 || ov > v || (ov == v && ow < who))) { v = ov; who = ow; }
+    // A continuation's place: those in front of it in its own beam, and of each other beam the larger ones (equal ones of an earlier beam too).  Where
+    // one of the best is nearer to another beam's continuation than their sums are known (32-bit exponentials: 2^-20 each), both beams' sums are taken
+    // again in 64 bits, until no such beams are left.
+    for (unsigned known = 0;;) {
+        for (int c = tid; c < p.beams * K; c += kMergeWarps * 32) {
+            if (token[c] < 0) continue;
+            const int mine = c / K;
+            const double v = total[c];
+            int rank = c - mine * K;
+            for (int i = 0; i < p.beams && rank < K; ++i) {
+                if (i == mine) continue;
+                int from = 0, to = K;                                           // the first of the beam that is not in front
+                while (from < to) {
+                    const int mid = (from + to) >> 1;
+                    const double other = total[i * K + mid];
+                    if (token[i * K + mid] >= 0 && (other > v || (other == v && i < mine))) from = mid + 1; else to = mid;
+                }
+                rank += from;
+            }
+            if (rank < K) { best[rank] = v; order[rank] = c; }
         }
-        const int t = __shfl_sync(0xffffffffu, has ? token[lane * K + at] : 0, who & 31);
-        if (lane == who) ++at;
-        if (lane == k) { best = v; parent = who & 31; chosen = t; }
+        if (tid == 0) near = 0;
+        __syncthreads();
+        for (int c = tid; c < p.beams * K; c += kMergeWarps * 32) {
+            if (token[c] < 0) continue;
+            for (int k = 0; k < K; ++k) {
+                const unsigned both = 1u << c / K | 1u << order[k] / K;
+                if (c / K != order[k] / K && fabs(best[k] - total[c]) < 0x1p-17 && (both & ~known)) atomicOr(&near, both & ~known);      // (-inf - -inf is not)
+            }
+        }
+        __syncthreads();
+        const unsigned again = near;
+        if (again == 0) break;
+        known |= again;
+        for (int i = 0; i < p.beams; ++i) {
+            const long long row = (long long)group * p.beams + i;
+            if (!(again >> i & 1) || (p.finished && p.finished[row])) continue;
+            const auto logit = [&](int v) {
+                return p.fp32 ? ((const float*)p.logits)[row * p.row_stride + v] : logit_of(((const bf16*)p.logits)[row * p.row_stride + v]);
+            };
+            float top = -INFINITY;
+            for (int v = tid; v < p.vocab; v += kMergeWarps * 32) top = fmaxf(top, logit(v));
+            top = warp_max(top);
+            if (lane == 0) partial[warp] = (double)top;
+            __syncthreads();
+            for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, (float)partial[w]);
+            double sum = 0.0;
+            for (int v = tid; v < p.vocab; v += kMergeWarps * 32) sum += exp((double)logit(v) - (double)top);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            __syncthreads();
+            if (lane == 0) partial[warp] = sum;
+            __syncthreads();
+            sum = 0.0;
+            for (int w = 0; w < kMergeWarps; ++w) sum += partial[w];
+            const double lse = (double)top + log(sum);
+            if (tid < K && token[i * K + tid] >= 0) total[i * K + tid] = (double)p.scores[row] + ((double)logit(token[i * K + tid]) - lse);
+            __syncthreads();
+        }
     }
+    __syncthreads();
+    if (warp) return;
+    const int chosen = lane < K ? order[lane] : 0, parent = chosen / K;
     int place = lane;
     if (p.placed) {
         // a beam's best continuation takes the beam's place, the others the places left, in order
-        const unsigned active = __ballot_sync(0xffffffffu, lane < K);
         const unsigned same = __match_any_sync(0xffffffffu, lane < K ? parent : 64 + lane);
         const bool leads = lane < K && (same & ((1u << lane) - 1u)) == 0;
         const unsigned taken = __reduce_or_sync(0xffffffffu, leads ? 1u << parent : 0u);
         const unsigned rest = __ballot_sync(0xffffffffu, lane < K && !leads);
-        (void)active;
         if (leads) place = parent;
         else {
             int skip = __popc(rest & ((1u << lane) - 1u));
@@ -181,58 +316,111 @@ __global__ void __launch_bounds__(kMergeWarps * 32) select_merge_kernel(const Se
     }
     if (lane < K) {
         const long long o = (long long)group * K + place;
-        p.scores_out[o] = (float)best;
+        p.scores_out[o] = (float)best[lane];
         p.parents_out[o] = group * p.beams + parent;
-        p.tokens_out[o] = chosen;
+        p.tokens_out[o] = token[chosen];
     }
 }
 
-// state[b] = old state[parents[b]] (-1: zeros; a row that is its own parent is not touched), for up to four tensors at once.  A block takes a column
-// of some bytes of all rows: it loads the rows that others copy, then writes, so that no row is read after it is overwritten.
+// state[b] = old state[parents[b]] (-1: zeros; a row that is its own parent is not touched), for up to four tensors at once.  A thread owns a column of
+// one unit of all rows, so nothing but its own order of reads and writes matters: a source that is itself overwritten is read first, into shared
+// memory; the others are read once and written to all their children.
 struct ReorderParams {
     char* state[4]; long long row[4]; long long stride[4]; long long slices[5];
     const int* parents; unsigned int* status;
-    int count, rows, width;                                   // tensors; sequences; units of a slice
+    int count, rows, held;                                    // tensors; sequences; bytes for rows that are read ahead
 };
+constexpr int kReorderThreads = 256, kReorderHeld = 24 * 1024, kReorderAtOnce = 4;
 template <typename U>
-__global__ void __launch_bounds__(256) reorder_kernel(const ReorderParams p) {
+__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderParams p) {
     grid_dependency_wait();            // without chain_enter(): kernels further on may fetch a state ahead of their own wait
     extern __shared__ __align__(16) unsigned char reorder_smem[];
-    U* held = reinterpret_cast<U*>(reorder_smem);                                          // [rows][width]
-    int* parents = reinterpret_cast<int*>(held + (size_t)p.rows * p.width);                // itself: not moved
-    int* needed = parents + p.rows;
-    const int tid = threadIdx.x;
-    for (int b = tid; b < p.rows; b += blockDim.x) {
-        int parent = p.parents[b];
-        if (parent < -1 || parent >= p.rows) { if (blockIdx.x == 0) atomicOr(p.status, QD_STATUS_BAD_ARG); parent = b; }
-        parents[b] = parent;
-        needed[b] = 0;
+    U* held = reinterpret_cast<U*>(reorder_smem);                                          // [source][thread]
+    int* first = reinterpret_cast<int*>(reorder_smem + p.held);                      // [rows + 2]: of each source (the last: zeros) its first child's place
+    int* child = first + p.rows + 2;                                                       // [rows]
+    int* source = child + p.rows;                                                          // [rows]: sources with children: from the front those that stay, from the back the others
+    __shared__ int stay, leave, sums[kReorderThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.rows;
+    const auto parent_of = [&](int b) {
+        const int parent = p.parents[b];
+        if (parent >= -1 && parent < S) return parent < 0 ? S : parent;
+        if (blockIdx.x == 0) atomicOr(p.status, QD_STATUS_BAD_ARG);
+        return b;
+    };
+    for (int i = tid; i < S + 2; i += kReorderThreads) first[i] = 0;
+    if (tid == 0) stay = leave = 0;
+    __syncthreads();
+    for (int b = tid; b < S; b += kReorderThreads) {
+        const int parent = parent_of(b);
+        if (parent != b) atomicAdd(first + parent + 1, 1);
     }
     __syncthreads();
-    for (int b = tid; b < p.rows; b += blockDim.x)
-        if (parents[b] >= 0 && parents[b] != b) needed[parents[b]] = 1;
+    int before = 0;                                           // counts to places
+    for (int base = 0; base < S + 2; base += kReorderThreads) {
+        const int i = base + tid;
+        int sum = i < S + 2 ? first[i] : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
+        }
+        if (lane == 31) sums[warp] = sum;
+        __syncthreads();
+        int all = 0;
+        for (int w = 0; w < kReorderThreads / 32; ++w) { if (w < warp) sum += sums[w]; all += sums[w]; }
+        if (i < S + 2) first[i] = before + sum;
+        before += all;
+        __syncthreads();
+    }
+    for (int b = tid; b < S; b += kReorderThreads) {
+        const int parent = parent_of(b);
+        if (parent != b) child[atomicAdd(first + parent, 1)] = b;           // (the order among the children changes nothing)
+    }
+    __syncthreads();
+    for (int i = tid; i < S; i += kReorderThreads) {                        // first[i] is now the end of source i's children, first[i - 1] their start
+        if (first[i] == (i ? first[i - 1] : 0)) continue;
+        if (parent_of(i) == i) source[atomicAdd(&stay, 1)] = i;
+        else source[S - 1 - atomicAdd(&leave, 1)] = i;
+    }
+    __syncthreads();
+    const int stays = stay, leaves = leave, zeros = S ? first[S - 1] : 0, zeros_end = first[S];
+    if (before == 0) return;
+    const int room = p.held / (int)sizeof(U), columns = leaves == 0 || room / leaves >= kReorderThreads ? kReorderThreads : room / leaves;
     for (long long slice = blockIdx.x; slice < p.slices[p.count]; slice += gridDim.x) {
         int t = 0;
         while (slice >= p.slices[t + 1]) ++t;
-        const long long first = (slice - p.slices[t]) * p.width, left = p.row[t] / (long long)sizeof(U) - first;
-        const int wide = (int)(left < p.width ? left : p.width);
-        __syncthreads();
-        for (int i = tid; i < p.rows * p.width; i += blockDim.x) {
-            const int b = i / p.width, c = i - b * p.width;
-            if (c < wide && needed[b]) held[i] = reinterpret_cast<const U*>(p.state[t] + b * p.stride[t])[first + c];
-        }
-        __syncthreads();
-        for (int i = tid; i < p.rows * p.width; i += blockDim.x) {
-            const int b = i / p.width, c = i - b * p.width, parent = parents[b];
-            if (c < wide && parent != b) reinterpret_cast<U*>(p.state[t] + b * p.stride[t])[first + c] = parent < 0 ? U{} : held[parent * p.width + c];
+        const long long units = p.row[t] / (long long)sizeof(U), from = (slice - p.slices[t]) * kReorderThreads;
+        const auto at = [&](int b, long long unit) -> U* { return reinterpret_cast<U*>(p.state[t] + b * p.stride[t]) + unit; };
+        for (int base = 0; base < kReorderThreads; base += columns) {      // (one round, unless many overwritten rows have to be held)
+            const long long unit = from + base + tid;
+            if (tid >= columns || base + tid >= kReorderThreads || unit >= units) continue;
+            for (int i = 0; i < leaves; ++i) held[i * columns + tid] = *at(source[S - 1 - i], unit);
+            for (int i = 0; i < stays; i += kReorderAtOnce) {
+                U x[kReorderAtOnce];
+#pragma unroll
+                for (int j = 0; j < kReorderAtOnce; ++j)
+                    if (i + j < stays) x[j] = *at(source[i + j], unit);
+#pragma unroll
+                for (int j = 0; j < kReorderAtOnce; ++j) {
+                    if (i + j >= stays) continue;
+                    const int who = source[i + j];
+                    for (int c = who ? first[who - 1] : 0; c < first[who]; ++c) *at(child[c], unit) = x[j];
+                }
+            }
+            for (int i = 0; i < leaves; ++i) {
+                const int who = source[S - 1 - i];
+                const U x = held[i * columns + tid];
+                for (int c = who ? first[who - 1] : 0; c < first[who]; ++c) *at(child[c], unit) = x;
+            }
+            for (int c = zeros; c < zeros_end; ++c) *at(child[c], unit) = U{};
         }
     }
 }
 
 template <typename U>
 int reorder_launch(const ReorderParams& p, dim3 grid, size_t smem, cudaStream_t stream) {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(reorder_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
-    return qd_launch(reorder_kernel<U>, grid, dim3(256), smem, stream, 3, p);
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(reorder_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
+    return qd_launch(reorder_kernel<U>, grid, dim3(kReorderThreads), smem, stream, 3, p);
 }
 
 int beam_sms() {
@@ -241,7 +429,7 @@ int beam_sms() {
     return sms > 0 ? sms : 148;
 }
 int splits_of(long long rows, int vocab) {
-    const long long want = beam_sms() / rows, most = vocab / 2048;
+    const long long want = beam_sms() * 8ll / rows, most = vocab / (kPartThreads * kPartEach);
     const long long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > kMostSplits ? kMostSplits : s);
 }
@@ -254,29 +442,38 @@ using namespace qd;
 extern "C" long long qd_beam_scratch_bytes(int batch, int beams, int vocab, int candidates) {
     if (batch <= 0 || beams <= 0 || vocab <= 0 || candidates <= 0) return 0;
     const long long rows = (long long)batch * beams;
-    return rows * splits_of(rows, vocab) * (candidates * 8ll + 8);
+    return rows * splits_of(rows, vocab) * (candidates * 8ll + 16);
 }
 
 extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_fp32, const float* scores, const void* finished, int eos, float* scores_out,
                               int* parents_out, void* tokens_out, void* scratch, int batch, int beams, int vocab, int candidates, int placed, void* stream) {
     QD_CHECK_ARG(logits && scores && scores_out && parents_out && tokens_out && scratch && batch > 0 && beams > 0 && vocab > 0 && candidates > 0);
     QD_CHECK_ARG((long long)beams * vocab >= candidates && (!finished || (eos >= 0 && eos < vocab)) && (!placed || candidates == beams));
-    QD_CHECK_ARG(((uintptr_t)scratch & 7u) == 0);
+    QD_CHECK_ARG(((uintptr_t)scratch & 15u) == 0);
     if (beams > kMostBeams || candidates > kMostBeams || (long long)batch * beams > 65535) return QD_ERR_UNSUPPORTED;
     SelectParams p;
     const long long rows = (long long)batch * beams;
     p.logits = logits; p.row_stride = row_stride; p.scores = scores; p.finished = (const uint8_t*)finished;
     p.splits = splits_of(rows, vocab);
-    p.keys = (unsigned long long*)scratch;
-    p.sums = (float2*)(p.keys + rows * p.splits * candidates);
+    p.sums = (double2*)scratch;
+    p.keys = (unsigned long long*)(p.sums + rows * p.splits);
     p.scores_out = scores_out; p.parents_out = parents_out; p.tokens_out = (long long*)tokens_out;
-    p.batch = batch; p.beams = beams; p.vocab = vocab; p.candidates = candidates; p.eos = eos; p.placed = placed;
-    int code = is_fp32 ? qd_launch(select_part_kernel<float>, dim3(p.splits, (unsigned)rows), dim3(kPartThreads), 0, (cudaStream_t)stream, 3, p)
-                       : qd_launch(select_part_kernel<bf16>, dim3(p.splits, (unsigned)rows), dim3(kPartThreads), 0, (cudaStream_t)stream, 3, p);
+    p.batch = batch; p.beams = beams; p.vocab = vocab; p.candidates = candidates; p.eos = eos; p.placed = placed; p.fp32 = is_fp32;
+    const int size = is_fp32 ? 4 : 2;
+    const bool whole = !(((uintptr_t)logits | (uintptr_t)(row_stride * size)) & 15u);
+    const size_t part = sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > 8 * candidates ? kPartMany : 8 * candidates));
+    const dim3 grid(p.splits, (unsigned)rows);
+    const cudaStream_t on = (cudaStream_t)stream;
+    int code;
+    if (whole) code = is_fp32 ? qd_launch(select_part_kernel<float, true>, grid, dim3(kPartThreads), part, on, 3, p)
+                              : qd_launch(select_part_kernel<bf16, true>, grid, dim3(kPartThreads), part, on, 3, p);
+    else code = is_fp32 ? qd_launch(select_part_kernel<float, false>, grid, dim3(kPartThreads), part, on, 3, p)
+                        : qd_launch(select_part_kernel<bf16, false>, grid, dim3(kPartThreads), part, on, 3, p);
     if (code != QD_OK) return code;
-    const size_t smem = (size_t)beams * candidates * 12 + (size_t)kMergeWarps * p.splits * candidates * 8;
+    const int lists = p.splits < candidates ? p.splits : candidates;
+    const size_t smem = (size_t)beams * candidates * 12 + (size_t)kMergeWarps * lists * candidates * 8;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
-    return qd_launch(select_merge_kernel, dim3(batch), dim3(kMergeWarps * 32), smem, (cudaStream_t)stream, 3, p);
+    return qd_launch(select_merge_kernel, dim3(batch), dim3(kMergeWarps * 32), smem, on, 3, p);
 }
 
 extern "C" int qd_reorder_states(void* state0, long long row0, long long stride0, void* state1, long long row1, long long stride1, void* state2,
@@ -298,13 +495,12 @@ extern "C" int qd_reorder_states(void* state0, long long row0, long long stride0
     if (p.count == 0) return QD_OK;
     p.parents = parents; p.status = status; p.rows = sequences;
     const int unit = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : align % 2 == 0 ? 2 : 1;
-    const long long room = 160 * 1024 - 8ll * sequences, width = room / ((long long)sequences * unit);
-    if (width < 1) return QD_ERR_UNSUPPORTED;
-    p.width = (int)(width < 512 / unit ? width : 512 / unit);
+    if (sequences > 7000) return QD_ERR_UNSUPPORTED;                         // (at least a column of every row is held)
+    p.held = 16 * sequences > kReorderHeld ? 16 * sequences : kReorderHeld;
+    const size_t smem = p.held + sizeof(int) * (3ull * sequences + 2);
     p.slices[0] = 0;
-    for (int i = 0; i < p.count; ++i) p.slices[i + 1] = p.slices[i] + (p.row[i] / unit + p.width - 1) / p.width;
-    const size_t smem = (size_t)sequences * p.width * unit + 8ull * sequences;
-    const long long most = (long long)beam_sms() * 8;
+    for (int i = 0; i < p.count; ++i) p.slices[i + 1] = p.slices[i] + (p.row[i] / unit + kReorderThreads - 1) / kReorderThreads;
+    const long long most = (long long)beam_sms() * (smem > 27 * 1024 ? 4 : 8);
     const dim3 grid((unsigned)(p.slices[p.count] < most ? p.slices[p.count] : most));
     const cudaStream_t on = (cudaStream_t)stream;
     return unit == 16 ? reorder_launch<uint4>(p, grid, smem, on) : unit == 4 ? reorder_launch<uint32_t>(p, grid, smem, on)
