@@ -9,13 +9,14 @@ namespace qd {
 namespace {
 
 constexpr int kBlocks = 8, kThreads = 1024, kWarps = kThreads / 32;
-enum { kMoves = 0, kCounts = 16, kCounts2 = 32, kLists = 48 };          // words of the scratch: number of moves, blocks' counts, lists
+enum { kMoves = 0, kCounts = 16, kMark = 24, kLists = 32 };             // words of the scratch: number of moves, blocks' counts, a number, lists
 
 struct Move { int from, to, rows; };
 
-QD_DEVINL void cluster_sync() {
+// BLOCKS 1: a block by itself, for what a block goes through in a few rounds; 8: a cluster.
+template <int BLOCKS> QD_DEVINL void all_sync() {
     __syncthreads();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (BLOCKS > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 QD_DEVINL int read_now(const int* p) { return __ldcg(p); }              // written by another block of the cluster
 
@@ -31,38 +32,58 @@ QD_DEVINL int block_before(int v, int* all, int* sums) {
     __syncthreads();                                                    // the previous use of `sums` is over
     if (lane == 31) sums[warp] = sum;
     __syncthreads();
-    int before = 0, total = 0;
-    for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
+    const int of = sums[lane];                                          // (a warp for every lane)
+    int before = lane < warp ? of : 0, total = of;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, d);
+        total += __shfl_xor_sync(0xffffffffu, total, d);
+    }
     *all = total;
     return before + sum - v;
 }
 
-// The places i of [first, last) with test(i), in ascending order, over all blocks of the cluster: found(rank, i) for ranks below `most`; how many
-// there are.  A block takes a run of places, a warp a run of the block's.  counts: kBlocks words, not used before in this launch.
-template <typename Test, typename Found>
-QD_DEVINL int cluster_list(int first, int last, int most, int* counts, int* sums, const Test& test, const Found& found) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, runs = kBlocks * kWarps;
-    const int per = ((last - first + runs - 1) / runs + 31) & ~31;
-    const int run = (int)blockIdx.x * kWarps + warp;
-    const long long from = first + (long long)run * per;
-    const int lo = (int)(from < last ? from : last), hi = (int)(from + per < last ? from + per : last);
+// The places i of [0, last) with test(i), in ascending order, over all blocks: a block takes a run of places, a warp a run of the block's.  After
+// `count` and a barrier, `before` is the number of such places in front of the warp's, `total` that of all.
+struct Run { int lo, hi, before, total; };
+template <int BLOCKS, typename Test>
+QD_DEVINL Run list_count(int last, int* counts, int* sums, const Test& test) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = ((last + BLOCKS * kWarps - 1) / (BLOCKS * kWarps) + 31) & ~31;
+    const long long from = (long long)((int)blockIdx.x * kWarps + warp) * per;
+    Run r;
+    r.lo = (int)(from < last ? from : last);
+    r.hi = (int)(from + per < last ? from + per : last);
     int mine = 0;
-    for (int base = lo; base < hi; base += 32) mine += __popc(__ballot_sync(0xffffffffu, base + lane < hi && test(base + lane)));
-    int all;
-    int rank = block_before(lane == 0 ? mine : 0, &all, sums);
-    if (threadIdx.x == 0) counts[blockIdx.x] = all;
-    cluster_sync();
-    int total = 0;
-    for (int b = 0; b < kBlocks; ++b) { const int c = read_now(counts + b); if (b < (int)blockIdx.x) rank += c; total += c; }
-    rank = __shfl_sync(0xffffffffu, rank, 0);
-    for (int base = lo; base < hi && rank < most; base += 32) {
-        const bool is = base + lane < hi && test(base + lane);
-        const unsigned all_of = __ballot_sync(0xffffffffu, is);
-        const int r = rank + __popc(all_of & ((1u << lane) - 1u));
-        if (is && r < most) found(r, base + lane);
-        rank += __popc(all_of);
+    for (int base = r.lo; base < r.hi; base += 32) mine += __popc(__ballot_sync(0xffffffffu, base + lane < r.hi && test(base + lane)));
+    r.before = __shfl_sync(0xffffffffu, block_before(lane == 0 ? mine : 0, &r.total, sums), 0);
+    if (BLOCKS > 1) {
+        if (threadIdx.x == 0) counts[blockIdx.x] = r.total;
+        all_sync<BLOCKS>();
+        const int all = lane < BLOCKS ? read_now(counts + lane) : 0;
+        int front = lane < (int)blockIdx.x ? all : 0, total = all;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            front += __shfl_xor_sync(0xffffffffu, front, d);
+            total += __shfl_xor_sync(0xffffffffu, total, d);
+        }
+        r.before += front;
+        r.total = total;
     }
-    return total;
+    return r;
+}
+// found(rank, i) for the warp's places with test(i), ranks below `most`.
+template <typename Test, typename Found>
+QD_DEVINL void list_found(const Run& r, int most, const Test& test, const Found& found) {
+    const int lane = threadIdx.x & 31;
+    int rank = r.before;
+    for (int base = r.lo; base < r.hi && rank < most; base += 32) {
+        const bool is = base + lane < r.hi && test(base + lane);
+        const unsigned all = __ballot_sync(0xffffffffu, is);
+        const int mine = rank + __popc(all & ((1u << lane) - 1u));
+        if (is && mine < most) found(mine, base + lane);
+        rank += __popc(all);
+    }
 }
 
 QD_DEVINL bool is_page(int e, int pages) { return e >= 0 && e < pages; }
@@ -72,167 +93,186 @@ struct ForkParams {
     int* table_out; int* lengths_out; int* refs_out; int* scratch; unsigned int* status;
     int sequences, width, pages, page;
 };
-// Rows and full pages of sequence b after the fork; `parent` is b itself where parents[b] names no sequence.
-struct Child { int parent, n, full, rest; bool stays, ends; };
-QD_DEVINL Child child_of(const ForkParams& p, int b) {
-    Child c;
-    const int parent = p.parents[b];
-    c.ends = parent == -1;
-    c.parent = parent < 0 || parent >= p.sequences ? b : parent;
-    c.stays = !c.ends && c.parent == b;
-    c.n = c.ends ? 0 : c.stays ? p.lengths[b] : min(max(p.lengths[c.parent], 0), p.width * p.page);
-    c.full = c.n / p.page;
-    c.rest = c.n - c.full * p.page;
-    return c;
-}
-
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) fork_kernel(const ForkParams p) {
-    chain_enter();
+// What concerns the sequences alone every block works out for itself, in shared memory; the blocks meet for the reference counts.
+template <int BLOCKS>
+QD_DEVINL void fork_pages(const ForkParams& p) {
+    extern __shared__ int fork_smem[];
     __shared__ int sums[kWarps];
-    const int tid = threadIdx.x, all = kBlocks * kThreads, at = blockIdx.x * kThreads + tid;
-    int* first = p.scratch + kLists;                                    // of each sequence: its first child, -1: itself
-    int* asks = first + p.sequences;                                    // sequences that need a page, in order
-    Move* moves = (Move*)(asks + p.sequences);
+    const int S = p.sequences, tid = threadIdx.x, all = BLOCKS * kThreads, at = blockIdx.x * kThreads + tid;
+    int *parent_of = fork_smem, *rows = parent_of + S, *first = rows + S, *asks = first + S;       // parent (itself where none is named; -1: ends), rows,
+    Move* moves = (Move*)(p.scratch + kLists);                                                    // first child (-1: itself), sequences that ask for a page
     for (int i = at; i < p.pages; i += all) p.refs_out[i] = p.refs[i];
-    for (int b = at; b < p.sequences; b += all) first[b] = p.sequences;
-    cluster_sync();
-    for (int b = at; b < p.sequences; b += all) {
-        const Child c = child_of(p, b);
+    for (int b = tid; b < S; b += kThreads) {
         const int parent = p.parents[b];
-        if (parent < -1 || parent >= p.sequences) atomicOr(p.status, QD_STATUS_BAD_ARG);
-        if (!c.ends) atomicMin(first + c.parent, c.stays ? -1 : b);
-        p.lengths_out[b] = c.n;
+        if (parent < -1 || parent >= S) { if (blockIdx.x == 0) atomicOr(p.status, QD_STATUS_BAD_ARG); }
+        parent_of[b] = parent < -1 || parent >= S ? b : parent;
+        rows[b] = p.lengths[b];
+        first[b] = S;
     }
-    // full pages shared, others dropped; a page that stays in its place needs no count
-    for (int b = blockIdx.x; b < p.sequences; b += kBlocks) {
-        const Child c = child_of(p, b);
-        for (int j = tid; j < p.width; j += kThreads) {
-            const int old = p.table[(long long)b * p.width + j];
-            const int now = c.stays ? old : j < c.full ? p.table[(long long)c.parent * p.width + j] : -1;
-            p.table_out[(long long)b * p.width + j] = now;
-            if (now != old) {
-                if (is_page(old, p.pages)) atomicSub(p.refs_out + old, 1);
-                if (is_page(now, p.pages)) atomicAdd(p.refs_out + now, 1);
-            }
+    all_sync<BLOCKS>();
+    for (int b = tid; b < S; b += kThreads)
+        if (parent_of[b] >= 0) atomicMin(first + parent_of[b], parent_of[b] == b ? -1 : b);
+    __syncthreads();
+    const auto length = [&](int b) {                                    // of b after the fork
+        const int parent = parent_of[b];
+        return parent < 0 ? 0 : parent == b ? rows[b] : min(max(rows[parent], 0), p.width * p.page);
+    };
+    // full pages shared, the page that is not full for the parent itself or its first child, others dropped; a page that stays in its place needs no count
+    for (long long i = at; i < (long long)S * p.width; i += all) {
+        const int b = (int)(i / p.width), j = (int)(i - (long long)b * p.width), parent = parent_of[b], old = p.table[i];
+        int now = old;
+        if (parent != b) {
+            const int n = length(b), full = n / p.page;
+            const bool mine = j < full || (j == full && n > full * p.page && first[parent] == b);
+            now = mine ? p.table[(long long)parent * p.width + j] : -1;
+        }
+        p.table_out[i] = now;
+        if (now != old) {
+            if (is_page(old, p.pages)) atomicSub(p.refs_out + old, 1);
+            if (is_page(now, p.pages)) atomicAdd(p.refs_out + now, 1);
         }
     }
-    cluster_sync();
-    // the page that is not full: to the parent itself or its first child, copies for the others
-    if (blockIdx.x == 0) {
-        int before = 0;
-        for (int base = 0; base < p.sequences; base += kThreads) {
-            const int b = base + tid;
-            bool asking = false;
-            if (b < p.sequences) {
-                const Child c = child_of(p, b);
-                if (!c.stays && c.rest > 0) {
-                    const int tail = p.table[(long long)c.parent * p.width + c.full];
-                    asking = read_now(first + c.parent) != b;
-                    if (!asking) {
-                        p.table_out[(long long)b * p.width + c.full] = tail;
-                        if (is_page(tail, p.pages)) atomicAdd(p.refs_out + tail, 1);
-                    }
-                }
-            }
-            int found;
-            const int rank = before + block_before(asking, &found, sums);
-            if (asking) asks[rank] = b;
-            before += found;
-        }
-        if (tid == 0) p.scratch[kMoves] = before;
+    int wanted = 0;
+    for (int base = 0; base < S; base += kThreads) {
+        const int b = base + tid, parent = b < S ? parent_of[b] : -1, n = b < S ? length(b) : 0;
+        const bool asking = parent >= 0 && parent != b && n % p.page != 0 && first[parent] != b;
+        if (b < S && blockIdx.x == 0) p.lengths_out[b] = n;
+        int found;
+        const int rank = wanted + block_before(asking, &found, sums);
+        if (asking) asks[rank] = b;
+        wanted += found;
     }
-    cluster_sync();
-    const int wanted = read_now(p.scratch + kMoves);
-    const int free = cluster_list(0, p.pages, wanted, p.scratch + kCounts, sums, [&](int i) { return read_now(p.refs_out + i) <= 0; },
-        [&](int rank, int page) {
-            const int b = read_now(asks + rank);
-            const Child c = child_of(p, b);
-            const int tail = p.table[(long long)c.parent * p.width + c.full];
-            p.table_out[(long long)b * p.width + c.full] = page;
-            moves[rank] = Move{tail, page, is_page(tail, p.pages) ? c.rest : 0};
-        });
-    cluster_sync();                                                     // all have read the counts and `wanted`
-    const int got = min(wanted, free);
-    for (int i = at; i < got; i += all) p.refs_out[read_now(&moves[i].to)] = 1;
-    for (int i = got + at; i < wanted; i += all) {                      // no page left: the sequence ends where its full pages do
-        const int b = read_now(asks + i);
-        p.lengths_out[b] = child_of(p, b).full * p.page;
+    all_sync<BLOCKS>();
+    const auto free_page = [&](int i) { return read_now(p.refs_out + i) <= 0; };
+    const Run run = list_count<BLOCKS>(p.pages, p.scratch + kCounts, sums, free_page);
+    list_found(run, wanted, free_page, [&](int rank, int page) {
+        const int b = asks[rank], parent = parent_of[b], n = length(b), full = n / p.page;
+        const int tail = p.table[(long long)parent * p.width + full];
+        p.table_out[(long long)b * p.width + full] = page;
+        p.refs_out[page] = 1;                                           // (looked at by this warp alone)
+        moves[rank] = Move{tail, page, is_page(tail, p.pages) ? n - full * p.page : 0};
+    });
+    if (blockIdx.x) return;
+    const int got = min(wanted, run.total);
+    for (int i = got + tid; i < wanted; i += kThreads) {                // no page left: the sequence ends where its full pages do
+        p.lengths_out[asks[i]] = length(asks[i]) / p.page * p.page;
         atomicOr(p.status, QD_STATUS_NO_PAGE);
     }
-    if (at == 0) p.scratch[kMoves] = got;
+    if (tid == 0) p.scratch[kMoves] = got;
+}
+__global__ void __launch_bounds__(kThreads) fork_block_kernel(const ForkParams p) {
+    chain_enter();
+    fork_pages<1>(p);
+}
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) fork_cluster_kernel(const ForkParams p) {
+    chain_enter();
+    fork_pages<kBlocks>(p);
 }
 
 struct CompactParams {
     const int* table; const int* refs; int* table_out; int* refs_out; int* used; int* scratch;
     int entries, pages, page;
 };
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) compact_kernel(const CompactParams p) {
-    chain_enter();
+template <int BLOCKS>
+QD_DEVINL void compact_pages(const CompactParams& p) {
     __shared__ int sums[kWarps];
-    const int tid = threadIdx.x, all = kBlocks * kThreads, at = blockIdx.x * kThreads + tid;
-    int* place = p.scratch + kLists;                                    // of each page: where it goes
+    const int tid = threadIdx.x, lane = tid & 31, all = BLOCKS * kThreads, at = blockIdx.x * kThreads + tid;
+    int* place = p.scratch + kLists;                                    // of a page that moves: where it goes
     Move* moves = (Move*)(place + p.pages);
-    const int used = cluster_list(0, p.pages, 0, p.scratch + kCounts, sums, [&](int i) { return p.refs[i] > 0; }, [](int, int) {});
-    for (int i = at; i < p.pages; i += all) { place[i] = i; p.refs_out[i] = p.refs[i]; }
-    cluster_list(0, used, p.pages, p.scratch + kCounts + kBlocks, sums, [&](int i) { return p.refs[i] <= 0; },
-                 [&](int rank, int i) { moves[rank].to = i; moves[rank].rows = p.page; });
-    const int count = cluster_list(used, p.pages, p.pages, p.scratch + kCounts2, sums, [&](int i) { return p.refs[i] > 0; },
-                                   [&](int rank, int i) { moves[rank].from = i; });
-    cluster_sync();
+    const auto taken = [&](int i) { return p.refs[i] > 0; };
+    const Run run = list_count<BLOCKS>(p.pages, p.scratch + kCounts, sums, taken);
+    const int used = run.total;
+    // pages in use among the first `used`: the warp that has the border counts to it
+    if (used == 0 && at == 0) p.scratch[kMark] = 0;
+    if (run.lo < used && run.hi >= used) {
+        int count = run.before;
+        for (int base = run.lo; base < used; base += 32) count += __popc(__ballot_sync(0xffffffffu, base + lane < used && taken(base + lane)));
+        if (lane == 0) p.scratch[kMark] = count;
+    }
+    all_sync<BLOCKS>();
+    const int front = read_now(p.scratch + kMark), count = used - front;
+    int rank = run.before;
+    for (int base = run.lo; base < run.hi; base += 32) {
+        const int i = base + lane, refs = i < run.hi ? p.refs[i] : 0;
+        const unsigned is = __ballot_sync(0xffffffffu, refs > 0);
+        const int in_front = rank + __popc(is & ((1u << lane) - 1u));
+        rank += __popc(is);
+        if (i >= run.hi) continue;
+        if (i < used && refs <= 0) { moves[i - in_front].to = i; moves[i - in_front].rows = p.page; }       // a free one: as many in front as are not in use
+        else if (i >= used && refs > 0) moves[in_front - front].from = i;
+        else p.refs_out[i] = refs;
+    }
+    all_sync<BLOCKS>();
     for (int i = at; i < count; i += all) {
         const int from = read_now(&moves[i].from), to = read_now(&moves[i].to);
         place[from] = to;
         p.refs_out[to] = p.refs[from];
         p.refs_out[from] = 0;
     }
-    cluster_sync();
+    all_sync<BLOCKS>();
     for (int i = at; i < p.entries; i += all) {
         const int e = p.table[i];
-        p.table_out[i] = is_page(e, p.pages) ? read_now(place + e) : e;
+        p.table_out[i] = e >= used && e < p.pages && p.refs[e] > 0 ? read_now(place + e) : e;
     }
     if (at == 0) { *p.used = used; p.scratch[kMoves] = count; }
+}
+__global__ void __launch_bounds__(kThreads) compact_block_kernel(const CompactParams p) {
+    chain_enter();
+    compact_pages<1>(p);
+}
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) compact_cluster_kernel(const CompactParams p) {
+    chain_enter();
+    compact_pages<kBlocks>(p);
 }
 
 struct ReserveParams {
     int* table; const int* lengths; int* refs; const int* counts; int* scratch; unsigned int* status;
     int count, sequences, width, pages, page;
 };
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) reserve_kernel(const ReserveParams p) {
-    chain_enter();
+// One block, or (many pages) a cluster whose blocks all list the requests.
+template <int BLOCKS>
+QD_DEVINL void reserve_pages(const ReserveParams& p) {
     __shared__ int sums[kWarps];
     const int tid = threadIdx.x;
     int* asks = p.scratch + kLists;                                     // places of the table that need a page, in order
-    if (blockIdx.x == 0) {
-        int before = 0;
-        for (int base = 0; base < p.sequences; base += kThreads) {
-            const int b = base + tid;
-            int from = 0, to = 0, need = 0;
-            if (b < p.sequences) {
-                const int n = p.lengths[b], more = p.counts ? p.counts[b] : p.count;
-                if (n < 0 || more < 0 || (long long)n + more > (long long)p.width * p.page) atomicOr(p.status, QD_STATUS_BAD_ARG);
-                else if (more > 0) {
-                    from = (n + p.page - 1) / p.page;
-                    to = (n + more + p.page - 1) / p.page;
-                    for (int j = from; j < to; ++j) need += p.table[(long long)b * p.width + j] < 0;
-                }
+    int wanted = 0;
+    for (int base = 0; base < p.sequences; base += kThreads) {
+        const int b = base + tid;
+        int from = 0, to = 0, need = 0;
+        if (b < p.sequences) {
+            const int n = p.lengths[b], more = p.counts ? p.counts[b] : p.count;
+            if (n < 0 || more < 0 || (long long)n + more > (long long)p.width * p.page) {
+                if (blockIdx.x == 0) atomicOr(p.status, QD_STATUS_BAD_ARG);
+            } else if (more > 0) {
+                from = (n + p.page - 1) / p.page;
+                to = (n + more + p.page - 1) / p.page;
+                for (int j = from; j < to; ++j) need += read_now(p.table + (long long)b * p.width + j) < 0;
             }
-            int found;
-            int rank = before + block_before(need, &found, sums);
-            for (int j = from; j < to; ++j)
-                if (p.table[(long long)b * p.width + j] < 0) asks[rank++] = b * p.width + j;
-            before += found;
         }
-        if (tid == 0) p.scratch[kMoves] = before;
+        int found;
+        int rank = wanted + block_before(need, &found, sums);
+        if (blockIdx.x == 0 && need > 0)
+            for (int j = from; j < to; ++j)
+                if (read_now(p.table + (long long)b * p.width + j) < 0) asks[rank++] = b * p.width + j;
+        wanted += found;
     }
-    cluster_sync();
-    const int wanted = read_now(p.scratch + kMoves);
     if (wanted == 0) return;                                            // (of all blocks alike)
-    const int free = cluster_list(0, p.pages, wanted, p.scratch + kCounts, sums, [&](int i) { return p.refs[i] <= 0; },
-        [&](int rank, int page) {
-            p.table[read_now(asks + rank)] = page;
-            p.refs[page] = 1;
-        });
-    if (free < wanted && blockIdx.x == 0 && tid == 0) atomicOr(p.status, QD_STATUS_NO_PAGE);
+    all_sync<BLOCKS>();
+    const auto free_page = [&](int i) { return read_now(p.refs + i) <= 0; };
+    const Run run = list_count<BLOCKS>(p.pages, p.scratch + kCounts, sums, free_page);
+    list_found(run, wanted, free_page, [&](int rank, int page) {
+        p.table[read_now(asks + rank)] = page;
+        p.refs[page] = 1;
+    });
+    if (run.total < wanted && blockIdx.x == 0 && tid == 0) atomicOr(p.status, QD_STATUS_NO_PAGE);
+}
+__global__ void __launch_bounds__(kThreads) reserve_block_kernel(const ReserveParams p) {
+    chain_enter();
+    reserve_pages<1>(p);
+}
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) reserve_cluster_kernel(const ReserveParams p) {
+    chain_enter();
+    reserve_pages<kBlocks>(p);
 }
 
 // The moves' rows, of every layer of both pools: a warp per 2 KB, four pieces of a lane in flight.
@@ -293,6 +333,8 @@ int sms_of() {
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     return sms > 0 ? sms : 148;
 }
+// What a block goes through in a few rounds.
+bool few(long long entries, long long pages) { return entries <= 8 * kThreads && pages <= 16 * kThreads; }
 bool whole_pieces(const void* a, const void* b, long long x, long long y, long long z) {
     return !(((uintptr_t)a | (uintptr_t)b) & 15u) && x % 16 == 0 && y % 16 == 0 && z % 16 == 0;
 }
@@ -309,7 +351,7 @@ using namespace qd;
 
 extern "C" long long qd_pages_scratch_words(int sequences, int width, int pages) {
     if (sequences <= 0 || width <= 0 || pages <= 0) return 0;
-    const long long fork = 5ll * sequences, compact = 4ll * pages, reserve = (long long)sequences * width;
+    const long long fork = 3ll * sequences, compact = 4ll * pages, reserve = (long long)sequences * width;
     return kLists + (fork > compact ? fork > reserve ? fork : reserve : compact > reserve ? compact : reserve);
 }
 
@@ -322,9 +364,18 @@ extern "C" int qd_pages_fork(void* k, void* v, long long page_bytes, long long l
     QD_CHECK_ARG(layer_bytes >= page * row_bytes && page_bytes >= layers * layer_bytes);
     if (!whole_pieces(k, v, page_bytes, layer_bytes, row_bytes)) return QD_ERR_UNSUPPORTED;
     ForkParams p{table, lengths, refs, parents, table_out, lengths_out, refs_out, scratch, status, sequences, width, pages, page};
-    const int code = qd_launch(fork_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
+    const size_t smem = 16ull * sequences;
+    if (smem > 200 * 1024) return QD_ERR_UNSUPPORTED;
+    const bool alone = few((long long)sequences * width, pages);
+    if (smem > 48 * 1024) {
+        const auto attribute = cudaFuncAttributeMaxDynamicSharedMemorySize;
+        if ((alone ? cudaFuncSetAttribute(fork_block_kernel, attribute, 200 * 1024) : cudaFuncSetAttribute(fork_cluster_kernel, attribute, 200 * 1024)) != cudaSuccess)
+            return QD_ERR_LAUNCH;
+    }
+    const int code = alone ? qd_launch(fork_block_kernel, dim3(1), dim3(kThreads), smem, (cudaStream_t)stream, 3, p)
+                           : qd_launch(fork_cluster_kernel, dim3(kBlocks), dim3(kThreads), smem, (cudaStream_t)stream, 3, p);
     if (code != QD_OK) return code;
-    return launch_moves(k, v, page_bytes, layer_bytes, row_bytes, layers, page, scratch, scratch + kLists + 2 * sequences, (cudaStream_t)stream);
+    return launch_moves(k, v, page_bytes, layer_bytes, row_bytes, layers, page, scratch, scratch + kLists, (cudaStream_t)stream);
 }
 
 extern "C" int qd_pages_compact(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, int layers, const int* table,
@@ -335,7 +386,8 @@ extern "C" int qd_pages_compact(void* k, void* v, long long page_bytes, long lon
     QD_CHECK_ARG(layer_bytes >= page * row_bytes && page_bytes >= layers * layer_bytes);
     if (!whole_pieces(k, v, page_bytes, layer_bytes, row_bytes)) return QD_ERR_UNSUPPORTED;
     CompactParams p{table, refs, table_out, refs_out, used, scratch, sequences * width, pages, page};
-    const int code = qd_launch(compact_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
+    const int code = few((long long)sequences * width, pages) ? qd_launch(compact_block_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, 3, p)
+                                                              : qd_launch(compact_cluster_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
     if (code != QD_OK) return code;
     return launch_moves(k, v, page_bytes, layer_bytes, row_bytes, layers, page, scratch, scratch + kLists + pages, (cudaStream_t)stream);
 }
@@ -345,7 +397,8 @@ extern "C" int qd_pages_reserve(int* table, const int* lengths, int* refs, const
     QD_CHECK_ARG(table && lengths && refs && scratch && status && (counts || count >= 0));
     QD_CHECK_ARG(sequences > 0 && width > 0 && pages > 0 && page > 0 && (long long)sequences * width <= 0x7fffffffll);
     ReserveParams p{table, lengths, refs, counts, scratch, status, count, sequences, width, pages, page};
-    return qd_launch(reserve_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
+    return few(sequences, pages) ? qd_launch(reserve_block_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, 3, p)
+                                 : qd_launch(reserve_cluster_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
 }
 
 extern "C" int qd_pages_rows(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, void* k_rows, void* v_rows,
