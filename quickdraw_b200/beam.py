@@ -6,8 +6,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import lib, ptr
-from .paged import PagedBatchState, _is_ids, device_status, launch
+from ._lib import ptr
+from .paged import PagedBatchState, _is_ids, device_status, launch, scratch_size
 from .state import DecodeState
 
 BF16 = torch.bfloat16
@@ -37,12 +37,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     placed = candidates is None
     count = beams if placed else candidates
     assert 0 < count <= MOST_BEAMS and count <= beams * vocab, "1 to 32 candidates, no more than there are continuations"
-    scores_out = torch.empty((batch, count), dtype=torch.float32, device=logits.device)
+    scores_out = scores.new_empty((batch, count))
     parents = torch.empty((batch, count), dtype=torch.int32, device=logits.device)
     tokens = torch.empty((batch, count), dtype=torch.long, device=logits.device)
-    scratch = torch.empty(lib().qd_beam_scratch_bytes(batch, beams, vocab, count), dtype=torch.uint8, device=logits.device)
+    scratch = scores.new_empty(scratch_size(device, "qd_beam_scratch_bytes", batch, beams, vocab, count) // 4)
     launch(logits, "qd_beam_select", ptr(logits), logits.stride(1) if beams > 1 else logits.stride(0), int(logits.dtype is torch.float32), ptr(scores),
-           ptr(finished), 0 if finished is None else int(eos), ptr(scores_out), ptr(parents), ptr(tokens), ptr(scratch), batch, beams, vocab, count, int(placed))
+           ptr(finished), 0 if finished is None else eos, ptr(scores_out), ptr(parents), ptr(tokens), ptr(scratch), batch, beams, vocab, count, int(placed))
     return scores_out, parents, tokens
 
 
@@ -56,13 +56,16 @@ def reorder_states(states, parents: torch.Tensor, *, status: torch.Tensor | None
     assert _is_ids(status, device, 1)
     rows = []
     for t in states:
-        assert t.get_device() == device and t.ndim >= 1 and t.shape[0] == count, "tensors [sequences, ...] on one device"
-        assert t[0].is_contiguous() and (count == 1 or t.stride(0) >= t[0].numel()), "contiguous rows that do not overlap"
+        shape, strides = t.shape, t.stride()
+        row = t.numel() // count
+        assert t.get_device() == device and len(shape) >= 1 and shape[0] == count, "tensors [sequences, ...] on one device"
+        assert (t.is_contiguous() or t[0].is_contiguous()) and (count == 1 or strides[0] >= row), "contiguous rows that do not overlap"
         size = t.element_size()
-        rows += [(ptr(t), t[0].numel() * size, t.stride(0) * size)] if t.numel() else []
-    for first in range(0, len(rows), 4):
-        some = rows[first:first + 4] + [(None, 0, 0)] * 4
-        launch(parents, "qd_reorder_states", *(x for row in some[:4] for x in row), ptr(parents), ptr(status), count)
+        if row:
+            rows += (ptr(t), row * size, strides[0] * size)
+    for first in range(0, len(rows), 12):
+        some = rows[first:first + 12]
+        launch(parents, "qd_reorder_states", *some, *(None, 0, 0) * (4 - len(some) // 3), ptr(parents), ptr(status), count)
 
 
 @torch.inference_mode()

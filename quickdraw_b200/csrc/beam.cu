@@ -3,7 +3,7 @@
 // A continuation of beam i by token v counts score[i] + x[i, v] - log sum_w exp x[i, w].  Within a beam the order is that of the logits, so a first
 // kernel takes, of each piece of a row, the largest logits, the maximum and the sum of exponentials, and a second one joins the pieces, adds up in 64
 // bits (sums of different beams lie next to one another) and merges the beams.
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace qd {
 namespace {
@@ -35,6 +35,11 @@ struct SelectParams {
     int batch, beams, vocab, candidates, splits, eos, placed, fp32;
 };
 
+QD_DEVINL float exp_base2(float x) {             // (results below 2^-126 are zero)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // Descending order of 32 keys, one a lane.
 QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 #pragma unroll
@@ -48,10 +53,10 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
     return key;
 }
 
-// A block per piece of a row, one pass: eight logits a thread at a time, their maximum and sum of exponentials, and a list of the keys above a bound that
+// A block per piece of a row, one pass: sixteen logits a thread at a time, their maximum and sum of exponentials, and a list of the keys above a bound that
 // `candidates` keys seen so far reach.  The bound comes from the first chunk (of each warp's 32 largest keys the candidates-th, of these the largest),
 // and again where more than a few threads have a key above it; it rises to the candidates-th of the list when that grows.
-constexpr int kPartThreads = 256, kPartEach = 8, kPartMany = 48, kPartList = 256;
+constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 48, kPartList = 3 * kMostBeams + 16;
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
     chain_enter();
@@ -65,25 +70,25 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     const int lo = (int)((long long)(p.vocab / 8) * split / p.splits) * 8;
     const int hi = split + 1 == p.splits ? p.vocab : (int)((long long)(p.vocab / 8) * (split + 1) / p.splits) * 8;
     if (tid == 0) count = 0;
-    // the thread's j-th logit of the chunk from `base`: two pieces of four of fp32, one of eight of bf16, or single ones
+    // the thread's j-th logit of the chunk from `base`: four pieces of 16 bytes of fp32, two of bf16, or single ones
     constexpr int kRun = !WHOLE ? 1 : sizeof(T) == 4 ? 4 : 8;
     const auto place = [&](int base, int j) { return base + j / kRun * (kRun * kPartThreads) + tid * kRun + j % kRun; };
     const auto fetch = [&](int base, float (&v)[kPartEach]) {
+        if (base + kPartThreads * kPartEach <= hi) {                            // (of all threads alike)
 #pragma unroll
-        for (int j = 0; j < kPartEach; j += kRun) {
-            const int i = place(base, j);
-            if (WHOLE && i + kRun <= hi) {
-                const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + i));
+            for (int j = 0; j < kPartEach; j += kRun) {
+                if (!WHOLE) { v[j] = logit_of(x[place(base, j)]); continue; }
+                const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + place(base, j)));
                 const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (sizeof(T) == 4) v[j + e] = __uint_as_float(w[e]);
-                    else { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+                    else { v[j + 2 * e] = __uint_as_float(w[e] << 16); v[j + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < kRun; ++e) v[j + e] = i + e < hi ? logit_of(x[i + e]) : -INFINITY;
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPartEach; ++j) v[j] = place(base, j) < hi ? logit_of(x[place(base, j)]) : -INFINITY;
         }
     };
     // the `K` largest of the list, in order: a thread counts for its keys how many are larger
@@ -97,8 +102,9 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     };
     unsigned long long* out = p.keys + ((long long)row * p.splits + split) * K;
     float top = -INFINITY, next[kPartEach];
-    double sum = 0.0;                  // of sums of eight: 32 bits would lose a ten-millionth with every few terms
+    double sum = 0.0;                  // of sums of sixteen: 32 bits would lose a ten-millionth with every few terms
     unsigned long long bound = 0;
+    float least = -INFINITY;           // the bound's logit
     fetch(lo, next);
     __syncthreads();
     for (int base = lo; base < hi; base += kPartThreads * kPartEach) {
@@ -106,44 +112,47 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
 #pragma unroll
         for (int j = 0; j < kPartEach; ++j) { v[j] = next[j]; most = fmaxf(most, v[j]); }
         if (base + kPartThreads * kPartEach < hi) fetch(base + kPartThreads * kPartEach, next);
-        if (most > top) { sum *= (double)exp2f((top - most) * 1.4426950408889634f); top = most; }
+        if (most > top) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
         const float shift = top == -INFINITY ? 0.f : top;
         float e[kPartEach];
 #pragma unroll
-        for (int j = 0; j < kPartEach; ++j) e[j] = exp2f((v[j] - shift) * 1.4426950408889634f);      // (NaN and infinity go on)
-        sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
-        // the thread's largest key; places behind the end have none
-        unsigned long long mine = 0;
-        if (most >= key_logit(bound) || bound == 0) {
+        for (int j = 0; j < kPartEach; ++j) e[j] = exp_base2((v[j] - shift) * 1.4426950408889634f);      // (NaN and infinity go on)
 #pragma unroll
-            for (int j = 0; j < kPartEach; ++j) {
-                const unsigned long long key = place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0;
-                mine = key > mine ? key : mine;
-            }
-        }
-        const int above = __syncthreads_count(mine > bound);
+        for (int d = kPartEach / 2; d > 0; d >>= 1)
+#pragma unroll
+            for (int j = 0; j < d; ++j) e[j] += e[j + d];
+        sum += (double)e[0];
+        const bool hit = most >= least;
+        const int above = __syncthreads_count(hit);
         if (above == 0) continue;
+        const auto key_of = [&](int j) { return place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0; };       // places behind the end: none
         if (above > kPartMany) {
-            const unsigned long long sorted = warp_sorted(mine, lane), kth = __shfl_sync(0xffffffffu, sorted, K - 1);
+            unsigned long long mine = 0;
+#pragma unroll
+            for (int j = 0; j < kPartEach; ++j) mine = key_of(j) > mine ? key_of(j) : mine;
+            const unsigned long long kth = __shfl_sync(0xffffffffu, warp_sorted(mine, lane), K - 1);
             if (lane == 0) bounds[warp] = kth ? kth - 1 : 0;
             __syncthreads();
 #pragma unroll
             for (int w = 0; w < kPartThreads / 32; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+            if (bound) least = key_logit(bound);
         }
-        if (mine > bound) {
+        if (hit) {
 #pragma unroll
-            for (int j = 0; j < kPartEach; ++j) {
-                const unsigned long long key = place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0;
-                if (key > bound) part_list[atomicAdd(&count, 1)] = key;
-            }
+            for (int j = 0; j < kPartEach; ++j)
+                if (v[j] >= least) {
+                    const unsigned long long key = key_of(j);
+                    if (key > bound) part_list[atomicAdd(&count, 1)] = key;
+                }
         }
         __syncthreads();
         const int n = count;
-        if (n > kPartList || (base == lo && n > 2 * K && hi - lo > 4 * kPartThreads * kPartEach)) {
+        if (n > 3 * K + 16) {                                                   // (a thread counts n keys: often and few is less than seldom and many)
             keep(out, n);                                                       // (the results' place serves as scratch)
             __syncthreads();
             if (tid < K) part_list[tid] = out[tid];
             bound = out[K - 1];
+            least = key_logit(bound);
             if (tid == 0) count = K;
             __syncthreads();
         }
@@ -419,17 +428,13 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderP
 
 template <typename U>
 int reorder_launch(const ReorderParams& p, dim3 grid, size_t smem, cudaStream_t stream) {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(reorder_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
+    static bool raised[kDevices];
+    if (smem > 48 * 1024 && !raise_smem(reorder_kernel<U>, 200 * 1024, raised)) return QD_ERR_LAUNCH;
     return qd_launch(reorder_kernel<U>, grid, dim3(kReorderThreads), smem, stream, 3, p);
 }
 
-int beam_sms() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
-}
 int splits_of(long long rows, int vocab) {
-    const long long want = beam_sms() * 8ll / rows, most = vocab / (kPartThreads * kPartEach);
+    const long long want = device_blocks() * 8ll / rows, most = vocab / 2048;
     const long long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > kMostSplits ? kMostSplits : s);
 }
@@ -461,7 +466,7 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
     p.batch = batch; p.beams = beams; p.vocab = vocab; p.candidates = candidates; p.eos = eos; p.placed = placed; p.fp32 = is_fp32;
     const int size = is_fp32 ? 4 : 2;
     const bool whole = !(((uintptr_t)logits | (uintptr_t)(row_stride * size)) & 15u);
-    const size_t part = sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > 8 * candidates ? kPartMany : 8 * candidates));
+    const size_t part = sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates));
     const dim3 grid(p.splits, (unsigned)rows);
     const cudaStream_t on = (cudaStream_t)stream;
     int code;
@@ -472,7 +477,8 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
     if (code != QD_OK) return code;
     const int lists = p.splits < candidates ? p.splits : candidates;
     const size_t smem = (size_t)beams * candidates * 12 + (size_t)kMergeWarps * lists * candidates * 8;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(select_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != cudaSuccess) return QD_ERR_LAUNCH;
+    static bool raised[kDevices];
+    if (smem > 48 * 1024 && !raise_smem(select_merge_kernel, 96 * 1024, raised)) return QD_ERR_LAUNCH;
     return qd_launch(select_merge_kernel, dim3(batch), dim3(kMergeWarps * 32), smem, on, 3, p);
 }
 
@@ -500,7 +506,7 @@ extern "C" int qd_reorder_states(void* state0, long long row0, long long stride0
     const size_t smem = p.held + sizeof(int) * (3ull * sequences + 2);
     p.slices[0] = 0;
     for (int i = 0; i < p.count; ++i) p.slices[i + 1] = p.slices[i] + (p.row[i] / unit + kReorderThreads - 1) / kReorderThreads;
-    const long long most = (long long)beam_sms() * (smem > 27 * 1024 ? 4 : 8);
+    const long long most = (long long)device_blocks() * (smem > 27 * 1024 ? 4 : 8);
     const dim3 grid((unsigned)(p.slices[p.count] < most ? p.slices[p.count] : most));
     const cudaStream_t on = (cudaStream_t)stream;
     return unit == 16 ? reorder_launch<uint4>(p, grid, smem, on) : unit == 4 ? reorder_launch<uint32_t>(p, grid, smem, on)

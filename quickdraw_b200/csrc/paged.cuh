@@ -4,6 +4,32 @@
 
 namespace qd {
 
+// Of the current device, asked for once: -1 where there is none.
+constexpr int kDevices = 64;
+static inline int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kDevices ? dev : -1;
+}
+static inline int device_blocks() {
+    static int known[kDevices];
+    const int dev = current_device();
+    if (dev < 0) return 148;
+    if (!known[dev]) {
+        int sms = 0;
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        known[dev] = sms > 0 ? sms : 148;
+    }
+    return known[dev];
+}
+// A kernel's limit of dynamic shared memory, raised once per device (`raised`: of this kernel).
+template <typename... KArgs>
+static inline bool raise_smem(void (*kernel)(KArgs...), size_t bytes, bool (&raised)[kDevices]) {
+    const int dev = current_device();
+    if (dev < 0) return false;
+    if (!raised[dev]) raised[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+    return raised[dev];
+}
+
 // A sequence is cut into parts by its own length, the number of (sequence, key/value head, chunk of heads) triples and that of workers alone, so that
 // its result does not depend on its neighbours: as if all of the batch were as long, so that they fill some rounds of workers in least time (a part
 // costs `kPagedFixed` units beside its own: its state is written, read and joined); of cuts that are within 1 / 16 of it the finest, because beside

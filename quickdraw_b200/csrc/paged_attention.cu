@@ -68,11 +68,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
     }
 }
 
-int paged_blocks() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
-}
 // Query heads at a time.
 int chunk_of(int group, bool fp32) {
     const int most = fp32 || group <= 8 ? 8 : 16;
@@ -91,14 +86,15 @@ struct Plan { int seqs, workers, unit; };          // sequences of a launch, gro
 Plan plan_of(int dim, int chunk, bool fp32) {
     return with_work(dim, chunk, fp32, [](auto* work) {
         using W = std::remove_pointer_t<decltype(work)>;
-        return Plan{W::kSeqs, paged_blocks() * PagedTiles<W>::kGroups, PagedTiles<W>::kStride};
+        return Plan{W::kSeqs, device_blocks() * PagedTiles<W>::kGroups, PagedTiles<W>::kStride};
     });
 }
 template <class W>
 int tiles_launch(const PagedParams& p, cudaStream_t stream) {
     constexpr int kSmem = PagedTiles<W>::kSmem;
-    if (cudaFuncSetAttribute(paged_tiles_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return QD_ERR_LAUNCH;
-    return qd_launch(paged_tiles_kernel<W>, dim3(paged_blocks()), dim3(PagedTiles<W>::kThreads), kSmem, stream, 3, p);
+    static bool raised[kDevices];
+    if (!raise_smem(paged_tiles_kernel<W>, kSmem, raised)) return QD_ERR_LAUNCH;
+    return qd_launch(paged_tiles_kernel<W>, dim3(device_blocks()), dim3(PagedTiles<W>::kThreads), kSmem, stream, 3, p);
 }
 
 // By the number of rows: 32 columns of a row a block, a row a block, a row a warp.
@@ -112,7 +108,7 @@ int join_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
 int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
     const int code = with_work(p.dim, p.chunk, fp32, [&](auto* work) { return tiles_launch<std::remove_pointer_t<decltype(work)>>(p, stream); });
     if (code != QD_OK) return code;
-    return fp32 ? join_launch<float>(p, paged_blocks(), stream) : join_launch<bf16>(p, paged_blocks(), stream);
+    return fp32 ? join_launch<float>(p, device_blocks(), stream) : join_launch<bf16>(p, device_blocks(), stream);
 }
 
 }  // namespace

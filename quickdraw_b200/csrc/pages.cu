@@ -3,7 +3,7 @@
 // Which page goes where is decided by one cluster of blocks (a barrier between its phases, no launch); a second launch, of the whole GPU, moves the
 // bytes.  A request for a page gets the lowest free one, in the order of the requests, so that tables do not depend on the order of any atomics
 // (reference counts are whole numbers: their sums do not either).
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace qd {
 namespace {
@@ -328,11 +328,6 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
     }
 }
 
-int sms_of() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
-}
 // What a block goes through in a few rounds.
 bool few(long long entries, long long pages) { return entries <= 8 * kThreads && pages <= 16 * kThreads; }
 bool whole_pieces(const void* a, const void* b, long long x, long long y, long long z) {
@@ -341,7 +336,7 @@ bool whole_pieces(const void* a, const void* b, long long x, long long y, long l
 int launch_moves(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, int layers, int page, const int* scratch,
                  const int* list, cudaStream_t stream) {
     MoveParams m{(char*)k, (char*)v, scratch, list, page_bytes, layer_bytes, row_bytes, layers, page};
-    return qd_launch(move_kernel, dim3(sms_of() * 8), dim3(256), 0, stream, 3, m);
+    return qd_launch(move_kernel, dim3(device_blocks() * 8), dim3(256), 0, stream, 3, m);
 }
 
 }  // namespace
@@ -367,11 +362,9 @@ extern "C" int qd_pages_fork(void* k, void* v, long long page_bytes, long long l
     const size_t smem = 16ull * sequences;
     if (smem > 200 * 1024) return QD_ERR_UNSUPPORTED;
     const bool alone = few((long long)sequences * width, pages);
-    if (smem > 48 * 1024) {
-        const auto attribute = cudaFuncAttributeMaxDynamicSharedMemorySize;
-        if ((alone ? cudaFuncSetAttribute(fork_block_kernel, attribute, 200 * 1024) : cudaFuncSetAttribute(fork_cluster_kernel, attribute, 200 * 1024)) != cudaSuccess)
-            return QD_ERR_LAUNCH;
-    }
+    static bool raised_block[kDevices], raised_cluster[kDevices];
+    if (smem > 48 * 1024 && !(alone ? raise_smem(fork_block_kernel, 200 * 1024, raised_block) : raise_smem(fork_cluster_kernel, 200 * 1024, raised_cluster)))
+        return QD_ERR_LAUNCH;
     const int code = alone ? qd_launch(fork_block_kernel, dim3(1), dim3(kThreads), smem, (cudaStream_t)stream, 3, p)
                            : qd_launch(fork_cluster_kernel, dim3(kBlocks), dim3(kThreads), smem, (cudaStream_t)stream, 3, p);
     if (code != QD_OK) return code;
@@ -410,6 +403,6 @@ extern "C" int qd_pages_rows(void* k, void* v, long long page_bytes, long long l
     if (count == 0) return QD_OK;
     RowsParams p{(char*)k, (char*)v, (char*)k_rows, (char*)v_rows, table, status, page_bytes, layer_bytes, row_bytes, rows_layer_bytes,
                  layers, page, pages, width, first, count, out};
-    const long long blocks = (2ll * layers * count + 7) / 8, most = sms_of() * 8;
+    const long long blocks = (2ll * layers * count + 7) / 8, most = device_blocks() * 8;
     return qd_launch(rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (cudaStream_t)stream, 3, p);
 }

@@ -18,6 +18,8 @@ outside the tensors is touched.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ._lib import call, lib, ptr, stream_of
@@ -37,14 +39,26 @@ def device_status(device) -> torch.Tensor:
     return word
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def launch(tensor: torch.Tensor, name: str, *args) -> None:
     """A library call on the device of ``tensor``, whichever is current."""
     index = tensor.get_device()
-    if index < 0 or index == torch.cuda.current_device():
+    if index < 0 or index == _current_device():
         call(name, *args, stream_of(tensor))
     else:
         with torch.cuda.device(index):
             call(name, *args, stream_of(tensor))
+
+
+@functools.lru_cache(maxsize=4096)
+def scratch_size(device: int, name: str, *sizes: int) -> int:
+    """What an entry point that computes a size says (these go by the device's number of SMs); a short call is as long as its host side."""
+    if device < 0 or device == _current_device():
+        return int(getattr(lib(), name)(*sizes))
+    with torch.cuda.device(device):
+        return int(getattr(lib(), name)(*sizes))
 
 
 def _is_ids(t, device, *shape) -> bool:
@@ -53,15 +67,14 @@ def _is_ids(t, device, *shape) -> bool:
 
 def _check_pools(k, v):
     """Pools [pages, layers, page, kv_heads, dim] whose pages are contiguous; the sizes in bytes that the kernels walk them by."""
-    assert k.is_cuda and k.ndim == 5 and k.shape == v.shape and k.dtype is v.dtype and k.get_device() == v.get_device(), "two pools of one shape, type and device"
-    pages, layers, page, heads, dim = k.shape
-    size = k.element_size()
-    row = heads * dim
-    for t in (k, v):
-        assert min(t.shape) > 0 and t.stride()[1:] == (page * row, row, dim, 1) and t.stride(0) >= layers * page * row, "the layers of a page are contiguous"
-    assert k.stride(0) == v.stride(0) or pages == 1, "the pools' pages lie alike"
-    assert row * size % 16 == 0 and k.stride(0) * size % 16 == 0 and (k.data_ptr() | v.data_ptr()) % 16 == 0, "rows of whole 16-byte pieces"
-    return k.stride(0) * size, page * row * size, row * size, layers
+    shape, strides = k.shape, k.stride()
+    assert k.is_cuda and len(shape) == 5 and shape == v.shape and k.dtype is v.dtype and k.get_device() == v.get_device(), "two pools of one shape, type and device"
+    pages, layers, page, heads, dim = shape
+    size, row, at = k.element_size(), heads * dim, ptr(k) | ptr(v)
+    assert pages * layers * page * row > 0 and strides[1:] == (page * row, row, dim, 1) and strides[0] >= layers * page * row, "the layers of a page are contiguous"
+    assert v.stride() == strides, "the pools' pages lie alike"
+    assert (at | row * size | strides[0] * size) % 16 == 0, "rows of whole 16-byte pieces"
+    return strides[0] * size, page * row * size, row * size, layers
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -75,41 +88,47 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table    int32 [batch, width], lengths int32 [batch], on the device; rows of entries that are no page are not seen
     scale    1 / sqrt(dim) unless given
     window   > 0: only the last ``window`` rows and the first ``sinks`` are seen (pages between them need not exist)"""
-    assert q.is_cuda and q.ndim == 3 and q.dtype in (BF16, torch.float32), "bf16 or fp32 queries [batch, heads, dim] on a CUDA device"
-    batch, heads, dim = q.shape
+    kind = q.dtype
+    assert q.is_cuda and q.ndim == 3 and kind in (BF16, torch.float32), "bf16 or fp32 queries [batch, heads, dim] on a CUDA device"
+    batch, heads, dim = shape = q.shape
     device = q.get_device()
     assert k_pages.ndim == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == dim, "pools [pages, page, kv_heads, dim]"
-    assert k_pages.dtype is q.dtype and v_pages.dtype is q.dtype and k_pages.get_device() == device and v_pages.get_device() == device
+    assert k_pages.dtype is kind and v_pages.dtype is kind and k_pages.get_device() == device and v_pages.get_device() == device
     pages, page, kv_heads, _ = k_pages.shape
     assert batch > 0 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and pages > 0 and page > 0
     assert 0 < dim <= 256 and dim % 8 == 0, "a head dimension of at most 256, a multiple of 8"
-    assert table.ndim == 2 and table.dtype is torch.int32 and table.shape[0] == batch and table.shape[1] > 0 and table.stride(1) == 1
-    assert table.get_device() == device and _is_ids(lengths, device, batch)
-    assert table.shape[1] * page < 2 ** 31 - 4096, "positions of 32 bits"
+    assert table.ndim == 2, "a table [batch, width]"
+    rows, width = table.shape
+    assert table.dtype is torch.int32 and rows == batch and width > 0 and table.stride(1) == 1 and table.get_device() == device
+    assert _is_ids(lengths, device, batch)
+    assert width * page < 2 ** 31 - 4096, "positions of 32 bits"
     assert window >= 0 and sinks >= 0 and (window > 0 or sinks == 0), "first rows stay visible beside a window"
-    page_stride, row_stride, head_stride, one = k_pages.stride()
-    size = q.element_size()
-    assert one == 1 and v_pages.stride() == k_pages.stride() and q.stride(2) == 1, "contiguous elements, pools with the same strides"
-    assert (k_pages.data_ptr() | v_pages.data_ptr() | page_stride * size | row_stride * size | head_stride * size) % 16 == 0, "whole 16-byte pieces"
+    page_stride, row_stride, head_stride, one = strides = k_pages.stride()
+    q_row, q_head, q_one = q.stride()
+    fp32 = kind is torch.float32
+    at_k, at_v = ptr(k_pages), ptr(v_pages)
+    assert one == 1 and v_pages.stride() == strides and q_one == 1, "contiguous elements, pools with the same strides"
+    assert (at_k | at_v | (page_stride | row_stride | head_stride) * (4 if fp32 else 2)) % 16 == 0, "whole 16-byte pieces"
     gate_row = gate_head = 0
     if gate is not None:
-        assert gate.shape == q.shape and gate.dtype is q.dtype and gate.get_device() == device and gate.stride(2) == 1
-        gate_row, gate_head = gate.stride(0), gate.stride(1)
-    out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-    partial = torch.empty(lib().qd_paged_attention_floats(batch, heads, kv_heads, dim), dtype=torch.float32, device=q.device)
-    launch(q, "qd_paged_attention", ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), page_stride, row_stride, head_stride, ptr(table),
-           table.stride(0), ptr(lengths), ptr(gate), gate_row, gate_head, ptr(out), ptr(partial), batch, heads, kv_heads, dim, pages, page, table.shape[1],
-           min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1), float(dim ** -0.5 if scale is None else scale), int(q.dtype is torch.float32))
+        gate_row, gate_head, gate_one = gate.stride()
+        assert gate.shape == shape and gate.dtype is kind and gate.get_device() == device and gate_one == 1
+    out = q.new_empty(shape)
+    floats = scratch_size(device, "qd_paged_attention_floats", batch, heads, kv_heads, dim)
+    partial = q.new_empty(floats if fp32 else 2 * floats)
+    launch(q, "qd_paged_attention", ptr(q), q_row, q_head, at_k, at_v, page_stride, row_stride, head_stride, ptr(table), table.stride(0), ptr(lengths),
+           ptr(gate), gate_row, gate_head, ptr(out), ptr(partial), batch, heads, kv_heads, dim, pages, page, width,
+           window if window < 2 ** 31 else 2 ** 31 - 1, sinks if sinks < 2 ** 31 else 2 ** 31 - 1, dim ** -0.5 if scale is None else scale, int(fp32))
     return out
 
 
 def _check_tables(table, refs, device):
-    assert table.ndim == 2 and _is_ids(table, device, *table.shape) and table.numel() > 0 and refs.ndim == 1 and _is_ids(refs, device, *refs.shape)
-    assert table.numel() < 2 ** 31 - 8192 and refs.numel() > 0
+    assert table.ndim == 2 and _is_ids(table, device, *table.shape) and refs.ndim == 1 and _is_ids(refs, device, *refs.shape)
+    assert 0 < table.numel() < 2 ** 31 - 8192 and refs.numel() > 0
 
 
 def _scratch(table, refs):
-    return torch.empty(lib().qd_pages_scratch_words(table.shape[0], table.shape[1], refs.numel()), dtype=torch.int32, device=table.device)
+    return table.new_empty(scratch_size(table.get_device(), "qd_pages_scratch_words", *table.shape, refs.numel()))
 
 
 def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, *,
@@ -142,7 +161,7 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     device, (pages, _, page, _, _) = k_pages.get_device(), k_pages.shape
     _check_tables(table, refs, device)
     assert refs.numel() == pages
-    table_out, refs_out, used = torch.empty_like(table), torch.empty_like(refs), torch.empty((), dtype=torch.int32, device=table.device)
+    table_out, refs_out, used = torch.empty_like(table), torch.empty_like(refs), table.new_empty(())
     launch(k_pages, "qd_pages_compact", ptr(k_pages), ptr(v_pages), page_bytes, layer_bytes, row_bytes, layers, ptr(table), ptr(refs), ptr(table_out),
            ptr(refs_out), ptr(used), ptr(_scratch(table, refs)), *table.shape, pages, page)
     return table_out, refs_out, used
