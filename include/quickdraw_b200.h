@@ -253,8 +253,9 @@ int qd_paged_prepare(const void* qg, const void* k_new, const void* v_new, const
  * times sigmoid(gate) where given; zeros for a sequence that sees nothing.  Strides in elements: q and gate by row and head,
  * the pools (alike) by page, row and head, the table by row.  bf16 or fp32 (is_fp32 = 1); dim at most 256 and a multiple of
  * 8, pools 16-byte aligned with strides of whole 16-byte pieces, else QD_ERR_UNSUPPORTED.  partial:
- * qd_paged_attention_floats floats. */
-long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim);
+ * qd_paged_attention_floats floats for sequences that see at most `positions` (width * page, or window + sinks if that is
+ * less; 0 floats: NULL). */
+long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim, int positions);
 int qd_paged_attention(const void* q, long long q_row, long long q_head, const void* k, const void* v, long long page_stride,
                        long long row_stride, long long head_stride, const int* table, long long table_stride,
                        const int* lengths, const void* gate, long long gate_row, long long gate_head, void* out,

@@ -79,7 +79,7 @@ SIGNATURES = {
     "qd_batch_attn_decode": [P, P, P, P, P, P, P, L, P, P, P, P, I, I, I, I, I, I, F, F, I, P],
     "qd_batch_attention": [P, P, P, P, P, P, P, L, P, P, P, P, P, I, I, I, I, I, I, F, F, I, P],
     "qd_paged_prepare": [P, P, P, P, P, P, P, L, P, P, P, I, I, I, I, I, I, I, I, F, F, P],
-    "qd_paged_attention_floats": [I, I, I, I],
+    "qd_paged_attention_floats": [I, I, I, I, I],
     "qd_paged_attention": [P, L, L, P, P, L, L, L, P, L, P, P, L, L, P, P, I, I, I, I, I, I, I, I, I, F, I, P],
     "qd_pages_scratch_words": [I, I, I],
     "qd_pages_fork": [P, P, L, L, L, I, P, P, P, P, P, P, P, P, P, I, I, I, I, P],

@@ -95,8 +95,13 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     const auto keep = [&](unsigned long long* into, int n) {
         for (int i = tid; i < n; i += kPartThreads) {
             const unsigned long long key = part_list[i];
-            int rank = 0;
-            for (int z = 0; z < n; ++z) rank += part_list[z] > key;
+            int rank = 0, z = 0;
+#pragma unroll 4
+            for (; z + 1 < n; z += 2) {
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(part_list + z);
+                rank += (two.x > key) + (two.y > key);
+            }
+            if (z < n) rank += part_list[z] > key;
             if (rank < K) into[rank] = key;
         }
     };
@@ -112,7 +117,8 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
 #pragma unroll
         for (int j = 0; j < kPartEach; ++j) { v[j] = next[j]; most = fmaxf(most, v[j]); }
         if (base + kPartThreads * kPartEach < hi) fetch(base + kPartThreads * kPartEach, next);
-        if (most > top) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
+        // (terms of up to e^8 lose nothing, and few chunks rescale)
+        if (most > top + 8.f) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
         const float shift = top == -INFINITY ? 0.f : top;
         float e[kPartEach];
 #pragma unroll

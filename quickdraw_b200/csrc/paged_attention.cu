@@ -107,7 +107,7 @@ int join_launch(const PagedParams& p, int blocks, cudaStream_t stream) {
 }
 int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
     const int code = with_work(p.dim, p.chunk, fp32, [&](auto* work) { return tiles_launch<std::remove_pointer_t<decltype(work)>>(p, stream); });
-    if (code != QD_OK) return code;
+    if (code != QD_OK || p.cuts.most == 0) return code;
     return fp32 ? join_launch<float>(p, device_blocks(), stream) : join_launch<bf16>(p, device_blocks(), stream);
 }
 
@@ -116,8 +116,8 @@ int paged_launch(const PagedParams& p, bool fp32, cudaStream_t stream) {
 
 using namespace qd;
 
-extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim) {
-    if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
+extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_heads, int dim, int positions) {
+    if (positions < 0 || batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
     const int group = heads / kv_heads;
     long long most = 0;
     for (int fp32 = 0; fp32 < 2; ++fp32) {
@@ -125,7 +125,7 @@ extern "C" long long qd_paged_attention_floats(int batch, int heads, int kv_head
         const Plan plan = plan_of(dim, chunk, fp32);
         for (const int some : {batch < plan.seqs ? batch : plan.seqs, batch % plan.seqs}) {          // whole launches and the last one
             if (!some) continue;
-            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, plan.workers).most * chunk * (dim + 2);
+            const long long pairs = (long long)some * kv_heads * chunks, floats = pairs * paged_cuts(pairs, plan.workers, (positions - 1ll) / plan.unit + 1).most * chunk * (dim + 2);
             if (floats > most) most = floats;
         }
     }
@@ -136,7 +136,7 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
                                   long long row_stride, long long head_stride, const int* table, long long table_stride, const int* lengths,
                                   const void* gate, long long gate_row, long long gate_head, void* out, float* partial, int batch, int heads,
                                   int kv_heads, int dim, int pages, int page, int width, int window, int sinks, float scale, int is_fp32, void* stream) {
-    QD_CHECK_ARG(q && k && v && table && lengths && out && partial);
+    QD_CHECK_ARG(q && k && v && table && lengths && out);
     QD_CHECK_ARG(batch > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && dim > 0 && pages > 0 && page > 0 && width > 0);
     QD_CHECK_ARG(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0) && (long long)width * page <= 0x7fffffffll - 4096 && heads <= 65535);
     if (dim > 256 || dim % 8) return QD_ERR_UNSUPPORTED;
@@ -156,7 +156,8 @@ extern "C" int qd_paged_attention(const void* q, long long q_row, long long q_he
     for (int b = 0; b < batch; b += plan.seqs) {                 // (the scratch is used again in stream order)
         p.batch = batch - b < plan.seqs ? batch - b : plan.seqs;
         const long long pairs = (long long)p.batch * kv_heads * p.chunks;
-        p.cuts = paged_cuts(pairs, plan.workers);
+        p.cuts = paged_cuts(pairs, plan.workers, ((p.window ? (long long)p.window + p.sinks : (long long)width * page) - 1) / plan.unit + 1);
+        QD_CHECK_ARG(partial || p.cuts.most == 0);
         p.stats = (float2*)(p.partial + pairs * p.cuts.most * p.chunk * dim);
         p.q = (const char*)q + b * q_row * size;
         p.gate = gate ? (const char*)gate + b * gate_row * size : nullptr;

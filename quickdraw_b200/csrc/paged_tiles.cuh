@@ -211,8 +211,14 @@ __global__ void __launch_bounds__(PagedTiles<W>::kThreads, 1) paged_tiles_kernel
                     den += weight * of[w].y;
                     sum.x += weight * v.x; sum.y += weight * v.y; sum.z += weight * v.z; sum.w += weight * v.w;
                 }
-                *reinterpret_cast<float4*>(p.partial + paged_place(p, a, h) * p.dim + f) = sum;
-                if (f == 0) p.stats[paged_place(p, a, h)] = make_float2(top, den);
+                if (p.cuts.most) {
+                    *reinterpret_cast<float4*>(p.partial + paged_place(p, a, h) * p.dim + f) = sum;
+                    if (f == 0) p.stats[paged_place(p, a, h)] = make_float2(top, den);
+                } else {
+                    const float v[4] = {sum.x, sum.y, sum.z, sum.w}, inverse = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) paged_put<T>(p, a.b, a.head0 + h, f + e, den == 0.f ? 0.f : v[e] * inverse);
+                }
             }
             meet();                                                                     // the states are read, the next queries there
         }

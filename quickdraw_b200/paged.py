@@ -113,9 +113,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if gate is not None:
         gate_row, gate_head, gate_one = gate.stride()
         assert gate.shape == shape and gate.dtype is kind and gate.get_device() == device and gate_one == 1
-    out = q.new_empty(shape)
-    floats = scratch_size(device, "qd_paged_attention_floats", batch, heads, kv_heads, dim)
-    partial = q.new_empty(floats if fp32 else 2 * floats)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    floats = scratch_size(device, "qd_paged_attention_floats", batch, heads, kv_heads, dim,
+                          min(width * page, window + sinks) if window else width * page)
+    partial = q.new_empty(floats if fp32 else 2 * floats) if floats else None
     launch(q, "qd_paged_attention", ptr(q), q_row, q_head, at_k, at_v, page_stride, row_stride, head_stride, ptr(table), table.stride(0), ptr(lengths),
            ptr(gate), gate_row, gate_head, ptr(out), ptr(partial), batch, heads, kv_heads, dim, pages, page, width,
            window if window < 2 ** 31 else 2 ** 31 - 1, sinks if sinks < 2 ** 31 else 2 ** 31 - 1, dim ** -0.5 if scale is None else scale, int(fp32))
