@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
 #pragma unroll
         for (int j = 0; j < kPartEach; ++j) { v[j] = next[j]; most = fmaxf(most, v[j]); }
         if (base + kPartThreads * kPartEach < hi) fetch(base + kPartThreads * kPartEach, next);
-        // (terms of up to e^8 lose nothing, and few chunks rescale)
-        if (most > top + 8.f) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
+        // (terms of up to e^2 lose nothing, and few chunks rescale)
+        if (most > top + 2.f) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
         const float shift = top == -INFINITY ? 0.f : top;
         float e[kPartEach];
 #pragma unroll
@@ -185,27 +185,53 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     }
 }
 
-// A block per group: a warp joins a beam's pieces, then all beams' continuations are put in order.
-constexpr int kMergeWarps = 8;
-__global__ void __launch_bounds__(kMergeWarps * 32) select_merge_kernel(const SelectParams p) {
+// The first block's shared memory, from any block of the cluster.
+QD_DEVINL uint32_t of_first_block(const void* mine) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(mine)));
+    return at;
+}
+QD_DEVINL void store_there(uint32_t at, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory"); }
+QD_DEVINL void store_there(uint32_t at, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+QD_DEVINL unsigned load_there(uint32_t at) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+QD_DEVINL void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// A cluster per group: a warp joins a beam's pieces, then the first block puts all beams' continuations in order.
+//
+// Sums of 32-bit exponentials (2^-22 each from the instruction, as much from its argument, twice that from sums of sixteen) leave a beam's log-sum-exp
+// known to 2^-20.  Where one of the best is nearer than 2^-18 to another beam's continuation, both beams' sums are taken again in 64 bits by all blocks,
+// until no such beams are left: the choice is then that of 64 bits.  Of 16 beams that happens to one group in some fifty.
+constexpr int kMergeBlocks = 8, kMergeThreads = 128;
+__global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThreads) select_merge_kernel(const SelectParams p) {
     chain_enter();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // waited for before the first access to another block's memory
     extern __shared__ __align__(16) unsigned char merge_smem[];
-    __shared__ double best[kMostBeams], partial[kMergeWarps];
+    __shared__ double best[kMostBeams], partial[kMostBeams][kMergeBlocks], piece[kMergeThreads / 32];
     __shared__ int order[kMostBeams];
     __shared__ unsigned near;
-    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates, lists = p.splits < K ? p.splits : K;
+    const int block = blockIdx.x % kMergeBlocks, group = blockIdx.x / kMergeBlocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int K = p.candidates, lists = p.splits < K ? p.splits : K;
     double* total = reinterpret_cast<double*>(merge_smem);                                  // [beams][K], descending
-    unsigned long long* list = reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)warp * lists * K;
-    int* token = reinterpret_cast<int*>(reinterpret_cast<unsigned long long*>(total + p.beams * K) + (size_t)kMergeWarps * lists * K);   // -1: none
-    for (int i = warp; i < p.beams; i += kMergeWarps) {
-        const long long row = (long long)group * p.beams + i;
-        const float score = p.scores[row];
-        const bool done = p.finished && p.finished[row];
-        const unsigned long long* keys = p.keys + row * p.splits * K;
-        const unsigned long long head = lane < p.splits && !done ? keys[lane * K] : 0;
-        double lse = 0.0;
-        bool counts = isfinite(score);
-        if (!done) {
+    int* token = reinterpret_cast<int*>(total + p.beams * K);                               // [beams][K], -1: none
+    unsigned long long* list = reinterpret_cast<unsigned long long*>(total + p.beams * K + (p.beams * K + 1) / 2) + (size_t)warp * lists * K;
+    const int mine = block + warp * kMergeBlocks;                                           // the warp's beam
+    const auto finished = [&](int i) { return p.finished && p.finished[(long long)group * p.beams + i]; };
+    const auto top_of = [&](int i) {                                                        // the largest logit of a beam (by a whole warp)
+        return warp_max(lane < p.splits ? (float)p.sums[((long long)group * p.beams + i) * p.splits + lane].x : -INFINITY);
+    };
+    double lse = 0.0;
+    bool counts = false;
+    int n = 0;
+    if (mine < p.beams) {
+        const long long row = (long long)group * p.beams + mine;
+        counts = isfinite(p.scores[row]);
+        if (!finished(mine)) {
+            const unsigned long long* keys = p.keys + row * p.splits * K;
+            const unsigned long long head = lane < p.splits ? keys[lane * K] : 0;
             const double2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_double2(-INFINITY, 0.0);
             const float top = warp_max((float)s.x);
             const bool odd = __any_sync(0xffffffffu, lane < p.splits && (s.x != s.x || s.y != s.y));
@@ -214,105 +240,128 @@ __global__ void __launch_bounds__(kMergeWarps * 32) select_merge_kernel(const Se
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             lse = (double)top + log(sum);
             counts = counts && !odd && isfinite(lse);
-        }
-        for (int k = lane; k < K; k += 32) {
-            // the end at no cost, and what never follows, in the order of the tokens
-            int t = k;
-            double v = -INFINITY;
-            if (done && counts) {
-                t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
-                if (k == 0) v = score;
-            }
-            total[i * K + k] = v;
-            token[i * K + k] = (done || !counts) && t < p.vocab ? t : -1;
-        }
-        __syncwarp();
-        if (done || !counts) continue;
-        // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
-        const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
-        int n = 0;
-        for (int k = lane; k < (p.splits * K + 31) / 32 * 32; k += 32) {
-            const unsigned long long key = k < p.splits * K ? keys[k] : 0;
-            const bool in = key && key >= bound;
-            const unsigned all = __ballot_sync(0xffffffffu, in);
-            if (in) list[n + __popc(all & ((1u << lane) - 1u))] = key;
-            n += __popc(all);
-        }
-        __syncwarp();
-        for (int k = lane; k < n; k += 32) {
-            const unsigned long long key = list[k];
-            int rank = 0;
-            for (int z = 0; z < n; ++z) rank += list[z] > key;
-            if (rank < K) {
-                total[i * K + rank] = (double)score + ((double)key_logit(key) - lse);
-                token[i * K + rank] = key_index(key);
-            }
-        }
-        __syncwarp();
-    }
-    __syncthreads();
-    // A continuation's place: those in front of it in its own beam, and of each other beam the larger ones (equal ones of an earlier beam too).  Where
-    // one of the best is nearer to another beam's continuation than their sums are known (32-bit exponentials: 2^-20 each), both beams' sums are taken
-    // again in 64 bits, until no such beams are left.
-    for (unsigned known = 0;;) {
-        for (int c = tid; c < p.beams * K; c += kMergeWarps * 32) {
-            if (token[c] < 0) continue;
-            const int mine = c / K;
-            const double v = total[c];
-            int rank = c - mine * K;
-            for (int i = 0; i < p.beams && rank < K; ++i) {
-                if (i == mine) continue;
-                int from = 0, to = K;                                           // the first of the beam that is not in front
-                while (from < to) {
-                    const int mid = (from + to) >> 1;
-                    const double other = total[i * K + mid];
-                    if (token[i * K + mid] >= 0 && (other > v || (other == v && i < mine))) from = mid + 1; else to = mid;
+            if (counts) {
+                // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
+                const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
+                for (int k = lane; k < (p.splits * K + 31) / 32 * 32; k += 32) {
+                    const unsigned long long key = k < p.splits * K ? keys[k] : 0;
+                    const bool in = key && key >= bound;
+                    const unsigned all = __ballot_sync(0xffffffffu, in);
+                    if (in) list[n + __popc(all & ((1u << lane) - 1u))] = key;
+                    n += __popc(all);
                 }
-                rank += from;
-            }
-            if (rank < K) { best[rank] = v; order[rank] = c; }
-        }
-        if (tid == 0) near = 0;
-        __syncthreads();
-        for (int c = tid; c < p.beams * K; c += kMergeWarps * 32) {
-            if (token[c] < 0) continue;
-            for (int k = 0; k < K; ++k) {
-                const unsigned both = 1u << c / K | 1u << order[k] / K;
-                if (c / K != order[k] / K && fabs(best[k] - total[c]) < 0x1p-17 && (both & ~known)) atomicOr(&near, both & ~known);      // (-inf - -inf is not)
+                __syncwarp();
             }
         }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (mine < p.beams) {
+        const uint32_t totals = of_first_block(total + mine * K), tokens = of_first_block(token + mine * K);
+        const double score = (double)p.scores[(long long)group * p.beams + mine];
+        if (finished(mine) || !counts)
+            for (int k = lane; k < K; k += 32) {
+                // the end at no cost, and what never follows, in the order of the tokens
+                int t = k;
+                double v = -INFINITY;
+                if (counts) {
+                    t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
+                    if (k == 0) v = score;
+                }
+                store_there(totals + k * 8, v);
+                store_there(tokens + k * 4, t < p.vocab ? t : -1);
+            }
+        else {
+            for (int k = lane; k < n; k += 32) {
+                const unsigned long long key = list[k];
+                int rank = 0;
+                for (int z = 0; z < n; ++z) rank += list[z] > key;
+                if (rank < K) {
+                    store_there(totals + rank * 8, score + ((double)key_logit(key) - lse));
+                    store_there(tokens + rank * 4, key_index(key));
+                }
+            }
+            for (int k = n + lane; k < K; k += 32) store_there(tokens + k * 4, -1);
+        }
+    }
+    __syncwarp();
+    cluster_sync();
+    for (unsigned known = 0;;) {
+        if (block == 0) {
+            // the best of the beams' heads, K times; a lane has a beam's list, of equal ones the first beam's is taken
+            if (warp == 0) {
+                int at = 0;
+                const auto head_of = [&]() -> unsigned long long {              // orders like the doubles; 0: none
+                    if (lane >= p.beams || at >= K || token[lane * K + at] < 0) return 0;
+                    const long long bits = __double_as_longlong(total[lane * K + at] + 0.0);
+                    return bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | 1ull << 63;
+                };
+                unsigned long long head = head_of();
+                for (int k = 0; k < K; ++k) {
+                    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32));
+                    const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32) == high ? (unsigned)head : 0u);
+                    const int who = __ffs(__ballot_sync(0xffffffffu, head == ((unsigned long long)high << 32 | low))) - 1;
+                    if (lane == who) {
+                        best[k] = total[lane * K + at];
+                        order[k] = lane * K + at;
+                        ++at;
+                        head = head_of();
+                    }
+                }
+            }
+            if (tid == 0) near = 0;
+            __syncthreads();
+            for (int c = tid; c < p.beams * K; c += kMergeThreads) {
+                if (token[c] < 0 || total[c] < best[K - 1] - 0x1p-17) continue;
+                for (int k = 0; k < K; ++k) {
+                    const unsigned both = 1u << c / K | 1u << order[k] / K;
+                    if (c / K != order[k] / K && fabs(best[k] - total[c]) < 0x1p-18 && (both & ~known)) atomicOr(&near, both & ~known);      // (-inf - -inf is not)
+                }
+            }
+        }
         __syncthreads();
-        const unsigned again = near;
+        cluster_sync();
+        const unsigned again = load_there(of_first_block(&near));
         if (again == 0) break;
         known |= again;
         for (int i = 0; i < p.beams; ++i) {
-            const long long row = (long long)group * p.beams + i;
-            if (!(again >> i & 1) || (p.finished && p.finished[row])) continue;
-            const auto logit = [&](int v) {
-                return p.fp32 ? ((const float*)p.logits)[row * p.row_stride + v] : logit_of(((const bf16*)p.logits)[row * p.row_stride + v]);
-            };
-            float top = -INFINITY;
-            for (int v = tid; v < p.vocab; v += kMergeWarps * 32) top = fmaxf(top, logit(v));
-            top = warp_max(top);
-            if (lane == 0) partial[warp] = (double)top;
-            __syncthreads();
-            for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, (float)partial[w]);
+            if (!(again >> i & 1) || finished(i)) continue;
+            const long long at = ((long long)group * p.beams + i) * p.row_stride;
+            const float top = top_of(i);
             double sum = 0.0;
-            for (int v = tid; v < p.vocab; v += kMergeWarps * 32) sum += exp((double)logit(v) - (double)top);
+            for (int v = (int)((long long)p.vocab * block / kMergeBlocks) + tid; v < (int)((long long)p.vocab * (block + 1) / kMergeBlocks); v += kMergeThreads)
+                sum += exp((double)(p.fp32 ? ((const float*)p.logits)[at + v] : logit_of(((const bf16*)p.logits)[at + v])) - (double)top);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane == 0) piece[warp] = sum;
             __syncthreads();
-            if (lane == 0) partial[warp] = sum;
+            if (tid == 0) {
+                for (int w = 1; w < kMergeThreads / 32; ++w) sum += piece[w];
+                store_there(of_first_block(&partial[i][block]), sum);
+            }
             __syncthreads();
-            sum = 0.0;
-            for (int w = 0; w < kMergeWarps; ++w) sum += partial[w];
-            const double lse = (double)top + log(sum);
-            if (tid < K && token[i * K + tid] >= 0) total[i * K + tid] = (double)p.scores[row] + ((double)logit(token[i * K + tid]) - lse);
+        }
+        cluster_sync();
+        if (block == 0) {
+            for (int i = warp; i < p.beams; i += kMergeThreads / 32) {
+                if (!(again >> i & 1) || finished(i)) continue;
+                const long long row = (long long)group * p.beams + i;
+                const float top = top_of(i);
+                double sum = 0.0;
+                for (int z = 0; z < kMergeBlocks; ++z) sum += partial[i][z];
+                const double exact = (double)top + log(sum);
+                for (int k = lane; k < K; k += 32) {
+                    const int t = token[i * K + k];
+                    if (t < 0) continue;
+                    const float logit = p.fp32 ? ((const float*)p.logits)[row * p.row_stride + t] : logit_of(((const bf16*)p.logits)[row * p.row_stride + t]);
+                    total[i * K + k] = (double)p.scores[row] + ((double)logit - exact);
+                }
+            }
             __syncthreads();
         }
     }
-    __syncthreads();
-    if (warp) return;
+    cluster_sync();                                                             // all have looked at `near`
+    if (block || warp) return;
     const int chosen = lane < K ? order[lane] : 0, parent = chosen / K;
     int place = lane;
     if (p.placed) {
@@ -482,10 +531,8 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
                         : qd_launch(select_part_kernel<bf16, false>, grid, dim3(kPartThreads), part, on, 3, p);
     if (code != QD_OK) return code;
     const int lists = p.splits < candidates ? p.splits : candidates;
-    const size_t smem = (size_t)beams * candidates * 12 + (size_t)kMergeWarps * lists * candidates * 8;
-    static bool raised[kDevices];
-    if (smem > 48 * 1024 && !raise_smem(select_merge_kernel, 96 * 1024, raised)) return QD_ERR_LAUNCH;
-    return qd_launch(select_merge_kernel, dim3(batch), dim3(kMergeWarps * 32), smem, on, 3, p);
+    const size_t smem = 8ull * (beams * candidates + (beams * candidates + 1) / 2 + (size_t)(kMergeThreads / 32) * lists * candidates);       // at most 44 KB
+    return qd_launch(select_merge_kernel, dim3(batch * kMergeBlocks), dim3(kMergeThreads), smem, on, 3, p);
 }
 
 extern "C" int qd_reorder_states(void* state0, long long row0, long long stride0, void* state1, long long row1, long long stride1, void* state2,

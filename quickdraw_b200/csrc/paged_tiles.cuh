@@ -131,17 +131,14 @@ __global__ void __launch_bounds__(PagedTiles<W>::kThreads, 1) paged_tiles_kernel
                 const int size = (there >> (at + 4 * four + lr) & 1) << 4;
                 static_loop<0, S::kRow / 128>([&](auto j) { cp_async16_at<4 * four * S::kRow + j * 128, j * 128>(four & 1 ? to_odd : to, src, size); });
             });
-        else                            // columns past the head dimension: zeros
-#pragma unroll 1
-            for (int four = 0; four < W::kTile; four += 4) {
-                const T* src = first + __shfl_sync(0xffffffffu, off, at + four + lr);
-                const int size = (there >> (at + four + lr) & 1) << 4;
-#pragma unroll
-                for (int j = 0; j < S::kRow / 128; ++j) {
-                    const bool in = 8 * j + lq < pieces;
-                    cp_async16((four & 4 ? to_odd : to) + four * S::kRow + j * 128, in ? src + j * 8 * kPiece : (const T*)pool, in ? size : 0);
-                }
-            }
+        else                            // columns past the head dimension: zeros (no byte is read there)
+            static_loop<0, W::kTile / 4>([&](auto four) {
+                const T* src = first + __shfl_sync(0xffffffffu, off, at + 4 * four + lr);
+                const int size = (there >> (at + 4 * four + lr) & 1) << 4;
+                static_loop<0, S::kRow / 128>([&](auto j) {
+                    cp_async16_at<4 * four * S::kRow + j * 128, j * 128>(four & 1 ? to_odd : to, src, 8 * j + lq < pieces ? size : 0);
+                });
+            });
         cp_async_commit();
     };
     constexpr uint32_t kMask = W::kTile == 32 ? ~0u : (1u << (W::kTile & 31)) - 1u;
