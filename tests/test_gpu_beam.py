@@ -53,6 +53,26 @@ def test_ties_go_to_the_lowest(cuda_device, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [100, 5000, 70001])
+def test_neighbours_that_32_bits_do_not_tell_apart(cuda_device, vocab, dtype):
+    """Beams with the same logits in another order, whose sums differ by rounding alone, and scores one step apart: the step decides."""
+    for seed in range(12):
+        g = torch.Generator().manual_seed(seed)
+        row = (torch.randn(vocab, generator=g) * 3).to(dtype)
+        logits = torch.stack([row[torch.randperm(vocab, generator=g)] for _ in range(6)])[None].cuda()
+        scores = torch.full((1, 6), -10.0)
+        for i in torch.randperm(6, generator=g).tolist()[:3]:
+            scores[0, i] = torch.nextafter(scores[0, i], torch.tensor(0.0 if seed % 2 else -20.0))
+        got = beam.beam_select(logits, scores.cuda(), candidates=12)
+        # beams of equal scores are told apart by the last bits of 64-bit sums alone: only the scores' order, and the tokens of each beam's best, are fixed
+        chosen = scores[0][got[1][0].cpu().long()]
+        value = row.double()[:, None].new_tensor([float(logits[0, p, t]) for p, t in zip(got[1][0].tolist(), got[2][0].tolist())]) + chosen.double()
+        assert bool((value[1:] <= value[:-1]).all()), seed
+        best = torch.sort((torch.stack([logits[0, i].cpu().double() + scores[0, i].double() for i in range(6)])).view(-1), descending=True).values[:12]
+        assert torch.equal(value, best), seed
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_what_is_no_continuation(cuda_device, dtype):
     g = torch.Generator().manual_seed(2)
     for vocab in (50, 5000):

@@ -109,6 +109,28 @@ def test_views_with_other_strides(cuda_device):
     assert torch.equal(paged.paged_attention(heads_first, k, v, table, n, gate=gate), want)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (24, 2, 128), (4, 2, 64), (7, 1, 80)])
+def test_queries_and_gates_anywhere(cuda_device, heads, kv_heads, dim, dtype):
+    """Rows that start off every boundary but their elements' own."""
+    q, k, v, table, n, _ = problem([90, 0, 333], heads, kv_heads, dim, 16, dtype)
+    gate = torch.randn((3, heads, dim), generator=torch.Generator().manual_seed(7)).to(dtype).cuda()
+    want = paged.paged_attention(q, k, v, table, n, gate=gate)
+    for shift in (1, 3):
+        off = [torch.zeros((3, heads, dim + 5), dtype=dtype, device="cuda")[:, :, shift:shift + dim] for _ in range(2)]
+        off[0].copy_(q), off[1].copy_(gate)
+        assert torch.equal(paged.paged_attention(off[0], k, v, table, n, gate=off[1]), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("width", [1, 16, 17, 64, 900])
+def test_short_sequences_of_short_and_long_tables(cuda_device, width, dtype):
+    """One launch or two, by what the table could hold."""
+    for heads, kv_heads, dim in ((16, 2, 256), (32, 1, 128), (4, 4, 64)):
+        *args, gate = problem([0, 1, 16, 9, 0], heads, kv_heads, dim, 16, dtype, width=width, gate=True)
+        check(paged.paged_attention(*args, gate=gate), *args, gate=gate)
+
+
 def test_a_sequence_does_not_depend_on_its_neighbours(cuda_device):
     q, k, v, table, n, _ = problem([700, 3, 1500, 64], 16, 2, 256, 64, BF16)
     first = paged.paged_attention(q, k, v, table, n)
@@ -117,9 +139,11 @@ def test_a_sequence_does_not_depend_on_its_neighbours(cuda_device):
     assert torch.equal(paged.paged_attention(q, k, v, table, n)[[0, 2]], first[[0, 2]])
 
 
-def test_more_sequences_than_a_launch_takes(cuda_device):
-    lengths = [(37 * b) % 50 for b in range(1500)]
-    *args, _ = problem(lengths, 2, 1, 64, 16, BF16)
+@pytest.mark.parametrize("count,heads,kv_heads,dim,dtype,width", [(1500, 2, 1, 64, BF16, None), (1100, 2, 1, 64, BF16, 40), (300, 2, 1, 64, F32, 40),
+                                                                 (200, 16, 1, 256, BF16, 40), (300, 3, 1, 40, F32, None)])
+def test_more_sequences_than_a_launch_takes(cuda_device, count, heads, kv_heads, dim, dtype, width):
+    lengths = [(37 * b) % 50 for b in range(count)]
+    *args, _ = problem(lengths, heads, kv_heads, dim, 16, dtype, width=width)
     check(paged.paged_attention(*args), *args)
 
 
@@ -194,6 +218,31 @@ def test_fork_of_many(cuda_device):
     got = paged.fork_pages(k, v, table, n, refs, torch.tensor(parents, dtype=torch.int32, device="cuda"))
     for a, b in zip((k, v, *got), want):
         assert torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7))
+
+
+def test_fork_compaction_and_reservation_of_large_tables(cuda_device):
+    """More entries and pages than one block goes through."""
+    g = torch.Generator().manual_seed(8)
+    lengths = torch.randint(0, 1600, (60,), generator=g).tolist()
+    parents = torch.randint(-1, 60, (60,), generator=g).tolist()
+    k, v, table, n, refs = plain.cache(lengths, 8, 1, 1, 8, BF16, seed=6, spare=30000, width=210)
+    want = plain.fork(k, v, table, n, refs, parents, 8)
+    got = paged.fork_pages(k, v, table, n, refs, torch.tensor(parents, dtype=torch.int32, device="cuda"))
+    for a, b in zip((k, v, *got), want):
+        assert torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7))
+    table, n, refs = got
+    held = int((table >= 0).sum())
+    free = (refs.cpu() <= 0).nonzero()[:, 0].tolist()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = table.clone()
+    paged.reserve_pages(table, n, refs, 8, 33, status=status)
+    fresh = table[before < 0]
+    assert int(status) == 0 and fresh[fresh >= 0].tolist() == free[:int((table >= 0).sum()) - held]
+    want = plain.compact(k, v, table, refs)
+    got = paged.compact_pages(k, v, table, refs)
+    for a, b in zip((k, v, *got[:2]), want):
+        assert torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7))
+    assert int(got[2]) == want[4]
 
 
 def test_fork_without_room_and_with_parents_that_are_none(cuda_device):
