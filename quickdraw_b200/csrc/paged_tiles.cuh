@@ -38,6 +38,13 @@ QD_DEVINL uint4 paged_load16(const bf16* src) {
 // Four warps take a part, every fourth tile each, through rings of their own whose slots hold the keys or the values of a tile: nothing in the loop
 // waits for another warp.  At the end of a part the four join their states (alone a warp would write four times as many, 8 KB each for eight heads of
 // 256) while the block's other groups keep the loads going.
+//
+// Long caches are bound by HBM: 4 sequences of 100 000 to 131 072 positions, 32 heads on 8 of 128, 1.82 GB in 284 us with the join (6.4 TB/s); 32 of 8192,
+// 16 on 2 of 256, 537 MB in 94.  Of other lengths (32 up to 8192, 282 MB, 57 us) a tenth goes to parts that end at different times; some 9 us go to the
+// launches, the lengths, the first look into the table and the first rows, one after the other.  What it took, us for those three: parts cut by blocks
+// whose warps joined by the tree, straight code that missed the instruction cache at every part 366 / - / 137; their states through the free slot 317 / 121
+// / 84; warps by themselves 293 / 103 / 74; copies by whole lines (64 bytes of eight rows an instruction cost a tenth) 280 / 104 / 65; four warps a part,
+// offsets in the instructions, rescaling only by 2^8: 283 / 94 / 60; largest parts first 282 / 94 / 56.
 constexpr int kPagedGroup = 4;
 template <class W> struct PagedTiles {
     static constexpr int kThreads = W::kWarps * 32, kGroups = W::kWarps / kPagedGroup, kSize = sizeof(typename W::Type), kSlots = 2 * W::kAhead + 1;
