@@ -295,7 +295,8 @@ int qd_pages_rows(void* k, void* v, long long page_bytes, long long layer_bytes,
  * (bytes, or NULL) has one continuation, eos, at no cost.  A beam whose score is not finite, or whose logits have no finite
  * log-sum-exp, has none; what is no continuation counts -inf.  Results [batch, candidates]: fp32 scores, int32 parents
  * b * beams + i, int64 tokens, best first; placed: a beam's best one in the beam's place, the others in the places left, in
- * order (candidates == beams).  beams and candidates at most 32.  scratch: qd_beam_scratch_bytes bytes, 16-byte aligned. */
+ * order (candidates == beams).  beams and candidates at most 32.  scratch: qd_beam_scratch_bytes bytes, 16-byte aligned
+ * (0: NULL). */
 long long qd_beam_scratch_bytes(int batch, int beams, int vocab, int candidates);
 int qd_beam_select(const void* logits, long long row_stride, int is_fp32, const float* scores, const void* finished, int eos,
                    float* scores_out, int* parents_out, void* tokens_out, void* scratch, int batch, int beams, int vocab,

@@ -39,7 +39,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     assert 0 < count <= MOST_BEAMS and count <= beams * vocab, "1 to 32 candidates, no more than there are continuations"
     scores_out = torch.empty_like(scores) if placed else scores.new_empty((batch, count))
     parents, tokens = torch.empty_like(scores_out, dtype=torch.int32), torch.empty_like(scores_out, dtype=torch.long)
-    scratch = scores.new_empty(scratch_size(device, "qd_beam_scratch_bytes", batch, beams, vocab, count) // 4)
+    size = scratch_size(device, "qd_beam_scratch_bytes", batch, beams, vocab, count)
+    scratch = scores.new_empty(size // 4) if size else None
     launch(logits, "qd_beam_select", ptr(logits), logits.stride(1) if beams > 1 else logits.stride(0), int(logits.dtype is torch.float32), ptr(scores),
            ptr(finished), 0 if finished is None else eos, ptr(scores_out), ptr(parents), ptr(tokens), ptr(scratch), batch, beams, vocab, count, int(placed))
     return scores_out, parents, tokens

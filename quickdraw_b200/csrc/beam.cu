@@ -60,17 +60,12 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 // list of its own took 52 (no barrier, but eight first chunks instead of one), lists of 256 keys 80; 256 threads 43.
 constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 48, kPartList = 3 * kMostBeams + 16;
 template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
-    chain_enter();
-    extern __shared__ __align__(16) unsigned long long part_list[];             // kPartList, and what a chunk can add: kPartMany threads' keys, or those of `candidates` lanes of each warp
+QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long long* part_list, unsigned long long* out) {
+    // part_list: kPartList, and what a chunk can add: kPartMany threads' keys, or those of K lanes of each warp.  out: the K largest keys, 0 behind the last
     __shared__ unsigned long long bounds[kPartThreads / 32];
     __shared__ double2 sums[kPartThreads / 32];
     __shared__ int count;
-    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates;
-    if (p.finished && p.finished[row]) return;
-    const T* x = (const T*)p.logits + row * p.row_stride;
-    const int lo = (int)((long long)(p.vocab / 8) * split / p.splits) * 8;
-    const int hi = split + 1 == p.splits ? p.vocab : (int)((long long)(p.vocab / 8) * (split + 1) / p.splits) * 8;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) count = 0;
     // the thread's j-th logit of the chunk from `base`: four pieces of 16 bytes of fp32, two of bf16, or single ones
     constexpr int kRun = !WHOLE ? 1 : sizeof(T) == 4 ? 4 : 8;
@@ -107,7 +102,6 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
             if (rank < K) into[rank] = key;
         }
     };
-    unsigned long long* out = p.keys + ((long long)row * p.splits + split) * K;
     float top = -INFINITY, next[kPartEach];
     double sum = 0.0;                  // of sums of sixteen: 32 bits would lose a ten-millionth with every few terms
     unsigned long long bound = 0;
@@ -180,11 +174,24 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) sums[warp].y = sum;
     __syncthreads();
-    if (tid == 0) {
-        double total = 0.0;
-        for (int w = 0; w < kPartThreads / 32; ++w) total += sums[w].y;
-        p.sums[(long long)row * p.splits + split] = make_double2((double)all, total);
-    }
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kPartThreads / 32; ++w) total += sums[w].y;
+    return make_double2((double)all, total);
+}
+static size_t part_bytes(int candidates) {
+    return sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates));
+}
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
+    chain_enter();
+    extern __shared__ __align__(16) unsigned long long select_list[];
+    const int row = blockIdx.y, split = blockIdx.x, each = p.vocab / 8;
+    if (p.finished && p.finished[row]) return;
+    const int lo = (int)((long long)each * split / p.splits) * 8, hi = split + 1 == p.splits ? p.vocab : (int)((long long)each * (split + 1) / p.splits) * 8;
+    const long long at = (long long)row * p.splits + split;
+    const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, lo, hi, p.candidates, select_list, p.keys + at * p.candidates);
+    if (threadIdx.x == 0) p.sums[at] = sum;
 }
 
 // The first block's shared memory, from any block of the cluster.
@@ -208,89 +215,52 @@ QD_DEVINL void cluster_sync() { asm volatile("barrier.cluster.arrive.release.ali
 // known to 2^-20.  Where one of the best is nearer than 2^-18 to another beam's continuation, both beams' sums are taken again in 64 bits by all blocks,
 // until no such beams are left: the choice is then that of 64 bits.  Of 16 beams that happens to one group in some fifty.
 constexpr int kMergeBlocks = 8, kMergeThreads = 128;
-__global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThreads) select_merge_kernel(const SelectParams p) {
-    chain_enter();
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // waited for before the first access to another block's memory
-    extern __shared__ __align__(16) unsigned char merge_smem[];
-    __shared__ double best[kMostBeams], partial[kMostBeams][kMergeBlocks], piece[kMergeThreads / 32];
-    __shared__ int order[kMostBeams];
-    __shared__ unsigned near;
-    const int block = blockIdx.x % kMergeBlocks, group = blockIdx.x / kMergeBlocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int K = p.candidates, lists = p.splits < K ? p.splits : K;
-    double* total = reinterpret_cast<double*>(merge_smem);                                  // [beams][K], descending
-    int* token = reinterpret_cast<int*>(total + p.beams * K);                               // [beams][K], -1: none
-    unsigned long long* list = reinterpret_cast<unsigned long long*>(total + p.beams * K + (p.beams * K + 1) / 2) + (size_t)warp * lists * K;
-    const int mine = block + warp * kMergeBlocks;                                           // the warp's beam
-    const auto finished = [&](int i) { return p.finished && p.finished[(long long)group * p.beams + i]; };
-    const auto top_of = [&](int i) {                                                        // the largest logit of a beam (by a whole warp)
-        return warp_max(lane < p.splits ? (float)p.sums[((long long)group * p.beams + i) * p.splits + lane].x : -INFINITY);
-    };
-    double lse = 0.0;
-    bool counts = false;
-    int n = 0;
-    if (mine < p.beams) {
-        const long long row = (long long)group * p.beams + mine;
-        counts = isfinite(p.scores[row]);
-        if (!finished(mine)) {
-            const unsigned long long* keys = p.keys + row * p.splits * K;
-            const unsigned long long head = lane < p.splits ? keys[lane * K] : 0;
-            const double2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_double2(-INFINITY, 0.0);
-            const float top = warp_max((float)s.x);
-            const bool odd = __any_sync(0xffffffffu, lane < p.splits && (s.x != s.x || s.y != s.y));
-            double sum = s.y == 0.0 ? 0.0 : s.y * exp(s.x - (double)top);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            lse = (double)top + log(sum);
-            counts = counts && !odd && isfinite(lse);
+struct MergeShared {                                          // of the first block, but for `piece`
+    double best[kMostBeams], partial[kMostBeams][kMergeBlocks], piece[kMergeThreads / 32];
+    int order[kMostBeams];
+    float top[kMostBeams];
+    unsigned near;
+};
+// What a beam has to offer, into the first block's lists: n of its largest keys, in any order, the K largest among them (by a warp).
+QD_DEVINL void offer(const SelectParams& p, MergeShared& shared, double* total, int* token, int group, int beam, bool finished, bool counts, float top, double lse,
+                     const unsigned long long* list, int n) {
+    const int K = p.candidates, lane = threadIdx.x & 31;
+    const uint32_t totals = of_first_block(total + beam * K), tokens = of_first_block(token + beam * K);
+    const double score = (double)p.scores[(long long)group * p.beams + beam];
+    if (lane == 0) store_there(of_first_block(&shared.top[beam]), __float_as_int(top));
+    if (finished || !counts) {
+        for (int k = lane; k < K; k += 32) {
+            // the end at no cost, and what never follows, in the order of the tokens
+            int t = k;
+            double v = -INFINITY;
             if (counts) {
-                // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
-                const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
-                for (int k = lane; k < (p.splits * K + 31) / 32 * 32; k += 32) {
-                    const unsigned long long key = k < p.splits * K ? keys[k] : 0;
-                    const bool in = key && key >= bound;
-                    const unsigned all = __ballot_sync(0xffffffffu, in);
-                    if (in) list[n + __popc(all & ((1u << lane) - 1u))] = key;
-                    n += __popc(all);
-                }
-                __syncwarp();
+                t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
+                if (k == 0) v = score;
+            }
+            store_there(totals + k * 8, v);
+            store_there(tokens + k * 4, t < p.vocab ? t : -1);
+        }
+    } else {
+        for (int k = lane; k < n; k += 32) {
+            const unsigned long long key = list[k];
+            int rank = 0;
+            for (int z = 0; z < n; ++z) rank += list[z] > key;
+            if (rank < K) {
+                store_there(totals + rank * 8, score + ((double)key_logit(key) - lse));
+                store_there(tokens + rank * 4, key_index(key));
             }
         }
+        for (int k = n + lane; k < K; k += 32) store_there(tokens + k * 4, -1);
     }
     __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (mine < p.beams) {
-        const uint32_t totals = of_first_block(total + mine * K), tokens = of_first_block(token + mine * K);
-        const double score = (double)p.scores[(long long)group * p.beams + mine];
-        if (finished(mine) || !counts)
-            for (int k = lane; k < K; k += 32) {
-                // the end at no cost, and what never follows, in the order of the tokens
-                int t = k;
-                double v = -INFINITY;
-                if (counts) {
-                    t = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
-                    if (k == 0) v = score;
-                }
-                store_there(totals + k * 8, v);
-                store_there(tokens + k * 4, t < p.vocab ? t : -1);
-            }
-        else {
-            for (int k = lane; k < n; k += 32) {
-                const unsigned long long key = list[k];
-                int rank = 0;
-                for (int z = 0; z < n; ++z) rank += list[z] > key;
-                if (rank < K) {
-                    store_there(totals + rank * 8, score + ((double)key_logit(key) - lse));
-                    store_there(tokens + rank * 4, key_index(key));
-                }
-            }
-            for (int k = n + lane; k < K; k += 32) store_there(tokens + k * 4, -1);
-        }
-    }
-    __syncwarp();
-    cluster_sync();
+}
+// The choice from all beams' lists, after a barrier of the cluster.
+QD_DEVINL void choose(const SelectParams& p, MergeShared& shared, double* total, int* token, int group, int block) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.candidates;
+    const auto finished = [&](int i) { return p.finished && p.finished[(long long)group * p.beams + i]; };
     for (unsigned known = 0;;) {
         if (block == 0) {
-            // the best of the beams' heads, K times; a lane has a beam's list, of equal ones the first beam's is taken
+            // the shared.best of the beams' heads, K times; a lane has a beam's list, of equal ones the first beam's is taken
             if (warp == 0) {
                 int at = 0;
                 const auto head_of = [&]() -> unsigned long long {              // orders like the doubles; 0: none
@@ -304,42 +274,42 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
                     const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32) == high ? (unsigned)head : 0u);
                     const int who = __ffs(__ballot_sync(0xffffffffu, head == ((unsigned long long)high << 32 | low))) - 1;
                     if (lane == who) {
-                        best[k] = total[lane * K + at];
-                        order[k] = lane * K + at;
+                        shared.best[k] = total[lane * K + at];
+                        shared.order[k] = lane * K + at;
                         ++at;
                         head = head_of();
                     }
                 }
             }
-            if (tid == 0) near = 0;
+            if (tid == 0) shared.near = 0;
             __syncthreads();
             for (int c = tid; c < p.beams * K; c += kMergeThreads) {
-                if (token[c] < 0 || total[c] < best[K - 1] - 0x1p-17) continue;
+                if (token[c] < 0 || total[c] < shared.best[K - 1] - 0x1p-17) continue;
                 for (int k = 0; k < K; ++k) {
-                    const unsigned both = 1u << c / K | 1u << order[k] / K;
-                    if (c / K != order[k] / K && fabs(best[k] - total[c]) < 0x1p-18 && (both & ~known)) atomicOr(&near, both & ~known);      // (-inf - -inf is not)
+                    const unsigned both = 1u << c / K | 1u << shared.order[k] / K;
+                    if (c / K != shared.order[k] / K && fabs(shared.best[k] - total[c]) < 0x1p-18 && (both & ~known)) atomicOr(&shared.near, both & ~known);      // (-inf - -inf is not)
                 }
             }
         }
         __syncthreads();
         cluster_sync();
-        const unsigned again = load_there(of_first_block(&near));
+        const unsigned again = load_there(of_first_block(&shared.near));
         if (again == 0) break;
         known |= again;
         for (int i = 0; i < p.beams; ++i) {
             if (!(again >> i & 1) || finished(i)) continue;
             const long long at = ((long long)group * p.beams + i) * p.row_stride;
-            const float top = top_of(i);
+            const float top = __uint_as_float(load_there(of_first_block(&shared.top[i])));
             double sum = 0.0;
             for (int v = (int)((long long)p.vocab * block / kMergeBlocks) + tid; v < (int)((long long)p.vocab * (block + 1) / kMergeBlocks); v += kMergeThreads)
                 sum += exp((double)(p.fp32 ? ((const float*)p.logits)[at + v] : logit_of(((const bf16*)p.logits)[at + v])) - (double)top);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            if (lane == 0) piece[warp] = sum;
+            if (lane == 0) shared.piece[warp] = sum;
             __syncthreads();
             if (tid == 0) {
-                for (int w = 1; w < kMergeThreads / 32; ++w) sum += piece[w];
-                store_there(of_first_block(&partial[i][block]), sum);
+                for (int w = 1; w < kMergeThreads / 32; ++w) sum += shared.piece[w];
+                store_there(of_first_block(&shared.partial[i][block]), sum);
             }
             __syncthreads();
         }
@@ -348,9 +318,9 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
             for (int i = warp; i < p.beams; i += kMergeThreads / 32) {
                 if (!(again >> i & 1) || finished(i)) continue;
                 const long long row = (long long)group * p.beams + i;
-                const float top = top_of(i);
+                const float top = shared.top[i];
                 double sum = 0.0;
-                for (int z = 0; z < kMergeBlocks; ++z) sum += partial[i][z];
+                for (int z = 0; z < kMergeBlocks; ++z) sum += shared.partial[i][z];
                 const double exact = (double)top + log(sum);
                 for (int k = lane; k < K; k += 32) {
                     const int t = token[i * K + k];
@@ -364,10 +334,10 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
     }
     cluster_sync();                                                             // all have looked at `near`
     if (block || warp) return;
-    const int chosen = lane < K ? order[lane] : 0, parent = chosen / K;
+    const int chosen = lane < K ? shared.order[lane] : 0, parent = chosen / K;
     int place = lane;
     if (p.placed) {
-        // a beam's best continuation takes the beam's place, the others the places left, in order
+        // a beam's shared.best continuation takes the beam's place, the others the places left, in shared.order
         const unsigned same = __match_any_sync(0xffffffffu, lane < K ? parent : 64 + lane);
         const bool leads = lane < K && (same & ((1u << lane) - 1u)) == 0;
         const unsigned taken = __reduce_or_sync(0xffffffffu, leads ? 1u << parent : 0u);
@@ -382,10 +352,96 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
     }
     if (lane < K) {
         const long long o = (long long)group * K + place;
-        p.scores_out[o] = (float)best[lane];
+        p.scores_out[o] = (float)shared.best[lane];
         p.parents_out[o] = group * p.beams + parent;
         p.tokens_out[o] = token[chosen];
     }
+}
+
+__global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThreads) select_merge_kernel(const SelectParams p) {
+    chain_enter();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // waited for before the first access to another block's memory
+    extern __shared__ __align__(16) unsigned char merge_smem[];
+    __shared__ MergeShared shared;
+    const int block = blockIdx.x % kMergeBlocks, group = blockIdx.x / kMergeBlocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int K = p.candidates, lists = p.splits < K ? p.splits : K;
+    double* total = reinterpret_cast<double*>(merge_smem);                                  // [beams][K], descending
+    int* token = reinterpret_cast<int*>(total + p.beams * K);                               // [beams][K], -1: none
+    unsigned long long* list = reinterpret_cast<unsigned long long*>(total + p.beams * K + (p.beams * K + 1) / 2) + (size_t)warp * lists * K;
+    const int beam = block + warp * kMergeBlocks;                                           // the warp's
+    const long long row = (long long)group * p.beams + beam;
+    const bool there = beam < p.beams, finished = there && p.finished && p.finished[row];
+    float top = -INFINITY;
+    double lse = 0.0;
+    bool counts = there && isfinite(p.scores[row]);
+    int n = 0;
+    if (there && !finished) {
+        const unsigned long long* keys = p.keys + row * p.splits * K;
+        const unsigned long long head = lane < p.splits ? keys[lane * K] : 0;
+        const double2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_double2(-INFINITY, 0.0);
+        top = warp_max((float)s.x);
+        const bool odd = __any_sync(0xffffffffu, lane < p.splits && (s.x != s.x || s.y != s.y));
+        double sum = s.y == 0.0 ? 0.0 : s.y * exp(s.x - (double)top);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        lse = (double)top + log(sum);
+        counts = counts && !odd && isfinite(lse);
+        // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
+        const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
+        for (int k = lane; counts && k < (p.splits * K + 31) / 32 * 32; k += 32) {
+            const unsigned long long key = k < p.splits * K ? keys[k] : 0;
+            const bool in = key && key >= bound;
+            const unsigned all = __ballot_sync(0xffffffffu, in);
+            if (in) list[n + __popc(all & ((1u << lane) - 1u))] = key;
+            n += __popc(all);
+        }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (there) offer(p, shared, total, token, group, beam, finished, counts, top, lse, list, n);
+    cluster_sync();
+    choose(p, shared, total, token, group, block);
+}
+
+// Rows of one chunk: the blocks of a group's cluster take its beams' rows themselves, one after the other, and no second launch is needed (which costs
+// the host 5 us with its scratch; on the device 500 tokens of 16 x 16 beams take 17.9 instead of 17.7 us, 4096 of 1 x 4 9.9 instead of 10.4, but of 16 x 16
+// 27 instead of 19).
+constexpr int kShortVocab = kPartThreads * kPartEach;
+template <typename T, bool WHOLE>
+__global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThreads) select_short_kernel(const SelectParams p) {
+    static_assert(kMergeThreads == kPartThreads, "a block is both");
+    chain_enter();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // waited for before the first access to another block's memory
+    extern __shared__ __align__(16) unsigned char merge_smem[];
+    __shared__ MergeShared shared;
+    constexpr int kRows = kMostBeams / kMergeBlocks;
+    __shared__ unsigned long long keys[kRows][kMostBeams];
+    __shared__ double2 sums[kRows];
+    const int block = blockIdx.x % kMergeBlocks, group = blockIdx.x / kMergeBlocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.candidates;
+    double* total = reinterpret_cast<double*>(merge_smem);                                  // [beams][K], descending
+    int* token = reinterpret_cast<int*>(total + p.beams * K);                               // [beams][K], -1: none
+    unsigned long long* list = reinterpret_cast<unsigned long long*>(merge_smem + (p.beams * K * 12 + 15) / 16 * 16);
+    const auto finished = [&](int i) { return p.finished && p.finished[(long long)group * p.beams + i]; };
+    for (int i = 0; block + i * kMergeBlocks < p.beams; ++i) {
+        const int beam = block + i * kMergeBlocks;
+        if (finished(beam)) continue;
+        const long long row = (long long)group * p.beams + beam;
+        const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, 0, p.vocab, K, list, keys[i]);
+        if (threadIdx.x == 0) sums[i] = sum;
+        __syncthreads();
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int beam = block + warp * kMergeBlocks;
+    if (beam < p.beams) {
+        const double2 s = finished(beam) ? make_double2(0.0, 1.0) : sums[warp];
+        const double lse = s.x + log(s.y);
+        const bool counts = isfinite(p.scores[(long long)group * p.beams + beam]) && isfinite(lse);
+        const int n = __popc(__ballot_sync(0xffffffffu, lane < K && keys[warp][lane] != 0));
+        offer(p, shared, total, token, group, beam, finished(beam), counts, (float)s.x, lse, keys[warp], n);
+    }
+    cluster_sync();
+    choose(p, shared, total, token, group, block);
 }
 
 // state[b] = old state[parents[b]] (-1: zeros; a row that is its own parent is not touched), for up to four tensors at once.  A thread owns a column of
@@ -503,14 +559,14 @@ int splits_of(long long rows, int vocab) {
 using namespace qd;
 
 extern "C" long long qd_beam_scratch_bytes(int batch, int beams, int vocab, int candidates) {
-    if (batch <= 0 || beams <= 0 || vocab <= 0 || candidates <= 0) return 0;
+    if (batch <= 0 || beams <= 0 || vocab <= kShortVocab || candidates <= 0) return 0;
     const long long rows = (long long)batch * beams;
     return rows * splits_of(rows, vocab) * (candidates * 8ll + 16);
 }
 
 extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_fp32, const float* scores, const void* finished, int eos, float* scores_out,
                               int* parents_out, void* tokens_out, void* scratch, int batch, int beams, int vocab, int candidates, int placed, void* stream) {
-    QD_CHECK_ARG(logits && scores && scores_out && parents_out && tokens_out && scratch && batch > 0 && beams > 0 && vocab > 0 && candidates > 0);
+    QD_CHECK_ARG(logits && scores && scores_out && parents_out && tokens_out && (scratch || vocab <= kShortVocab) && batch > 0 && beams > 0 && vocab > 0 && candidates > 0);
     QD_CHECK_ARG((long long)beams * vocab >= candidates && (!finished || (eos >= 0 && eos < vocab)) && (!placed || candidates == beams));
     QD_CHECK_ARG(((uintptr_t)scratch & 15u) == 0);
     if (beams > kMostBeams || candidates > kMostBeams || (long long)batch * beams > 65535) return QD_ERR_UNSUPPORTED;
@@ -524,9 +580,17 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
     p.batch = batch; p.beams = beams; p.vocab = vocab; p.candidates = candidates; p.eos = eos; p.placed = placed; p.fp32 = is_fp32;
     const int size = is_fp32 ? 4 : 2;
     const bool whole = !(((uintptr_t)logits | (uintptr_t)(row_stride * size)) & 15u);
-    const size_t part = sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates));
+    const size_t part = part_bytes(candidates);
     const dim3 grid(p.splits, (unsigned)rows);
     const cudaStream_t on = (cudaStream_t)stream;
+    if (vocab <= kShortVocab) {
+        const size_t both = part + (beams * candidates * 12 + 15) / 16 * 16;          // at most 30 KB
+        const dim3 clusters(batch * kMergeBlocks);
+        if (whole) return is_fp32 ? qd_launch(select_short_kernel<float, true>, clusters, dim3(kMergeThreads), both, on, 3, p)
+                                  : qd_launch(select_short_kernel<bf16, true>, clusters, dim3(kMergeThreads), both, on, 3, p);
+        return is_fp32 ? qd_launch(select_short_kernel<float, false>, clusters, dim3(kMergeThreads), both, on, 3, p)
+                       : qd_launch(select_short_kernel<bf16, false>, clusters, dim3(kMergeThreads), both, on, 3, p);
+    }
     int code;
     if (whole) code = is_fp32 ? qd_launch(select_part_kernel<float, true>, grid, dim3(kPartThreads), part, on, 3, p)
                               : qd_launch(select_part_kernel<bf16, true>, grid, dim3(kPartThreads), part, on, 3, p);

@@ -278,8 +278,9 @@ class PagedBatchState:
 
     def __init__(self, config, batch: int, max_context: int, device, pages: int | None = None, page: int = 64):
         one = DecodeState.allocate(config, 1, "meta")
-        self.cache = PagedCache(one.kv_k.shape[0], config.num_key_value_heads, config.head_dim, pages or batch * -(-max_context // page), page, batch,
-                                max_context, device)
+        enough = batch * -(-max_context // page)
+        self.cache = PagedCache(one.kv_k.shape[0], config.num_key_value_heads, config.head_dim, enough if pages is None else pages, page, batch, max_context,
+                                device)
         self.rec_state = torch.zeros((batch, *one.rec_state.shape), dtype=torch.float32, device=device)
         self.conv_state = torch.zeros((batch, *one.conv_state.shape), dtype=BF16, device=device)
         self.positions = self.cache.lengths

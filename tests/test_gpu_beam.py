@@ -24,7 +24,7 @@ def same(got, logits, scores, **kwargs):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("batch,beams,vocab", [(1, 1, 1), (1, 1, 40), (2, 4, 5), (3, 5, 1000), (1, 4, 151936), (2, 16, 4097), (1, 32, 33), (7, 3, 20000), (40, 8, 515)])
+@pytest.mark.parametrize("batch,beams,vocab", [(1, 1, 1), (1, 1, 40), (2, 4, 5), (3, 5, 1000), (1, 4, 151936), (2, 16, 4097), (1, 32, 33), (7, 3, 20000), (40, 8, 515), (3, 32, 2048), (3, 12, 2049)])
 def test_select(cuda_device, batch, beams, vocab, dtype):
     g = torch.Generator().manual_seed(vocab)
     logits = (torch.randn((batch, beams, vocab), generator=g) * 3).to(dtype).cuda()

@@ -118,6 +118,11 @@ def test_cache_of_no_size_is_refused():
     assert cache.table.shape == (3, 7) and bool((cache.table == -1).all()) and cache.pages == 4 and cache.check() == 0
     with pytest.raises(AssertionError):
         cache.free([3])
+    config = synthetic.model_config(num_layers=4, vocab_size=64)
+    with pytest.raises(AssertionError):
+        paged.PagedBatchState(config, 2, 64, "cpu", pages=0)
+    state = paged.PagedBatchState(config, 2, 65, "cpu", page=16)
+    assert state.cache.pages == 10 and state.cache.k.shape == (10, 1, 16, 2, 256) and state.positions is state.cache.lengths
 
 
 def test_select_passes_its_arguments(calls):
