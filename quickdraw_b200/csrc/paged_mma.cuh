@@ -35,7 +35,8 @@ template <int D, int NT> struct PagedMma {
     static constexpr int kSeqs = D == 256 && NT == 2 ? 192 : 1024;     // (what memory has room for)
     const int lane, g, t;
     const uint32_t key_turn, value_turn;
-    uint32_t q_row, q4[NT == 1 ? D / 32 : 1][4];                       // eight heads are kept in registers, sixteen read again for each tile
+    static constexpr bool kHeld = NT == 1 || D == 128;                 // queries in registers (24 heads of 128 on a key head, 28 x 12307 positions: 122.7 us, 130.5 read for each tile); sixteen heads of 64 or 256 find no room
+    uint32_t q_row, q4[kHeld ? NT * D / 32 : 1][4];
     float acc[NT][D / 16][4], m[NT][2], l[NT][2];                      // columns g and g + 8 of every sixteen, heads 2 t and 2 t + 1
     uint32_t hi[NT][2], lo[NT][2];
 
@@ -45,9 +46,11 @@ template <int D, int NT> struct PagedMma {
 
     QD_DEVINL void begin(uint32_t queries) {
         q_row = queries + (lane & 7) * (D * 2);
-        if (NT == 1) {
+        if (kHeld) {
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) ldmatrix4(q4[k], q_row + (((4 * k + (lane >> 3)) ^ (lane & 7)) << 4));
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) ldmatrix4(q4[n * D / 32 + k], q_row + n * 8 * (D * 2) + (((4 * k + (lane >> 3)) ^ (lane & 7)) << 4));
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -75,8 +78,8 @@ template <int D, int NT> struct PagedMma {
             ldmatrix4<(k >> 1) * 128>(kb, at ^ 32);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                uint32_t (&q)[4] = q4[NT == 1 ? (int)k : 0];
-                if (NT > 1) ldmatrix4(q, q_row + n * 8 * (D * 2) + (((4 * k + (lane >> 3)) ^ (lane & 7)) << 4));
+                uint32_t (&q)[4] = q4[kHeld ? n * D / 32 + k : 0];
+                if (!kHeld) ldmatrix4(q, q_row + n * 8 * (D * 2) + (((4 * k + (lane >> 3)) ^ (lane & 7)) << 4));
                 mma16816(s[n][0], ka, q[0], q[1]);
                 mma16816(s[n][1], kb, q[2], q[3]);
             }
