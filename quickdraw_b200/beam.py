@@ -63,6 +63,7 @@ def reorder_states(states, parents: torch.Tensor, *, status: torch.Tensor | None
         size = t.element_size()
         if row:
             rows += (ptr(t), row * size, strides[0] * size)
+    assert 3 * len(set(rows[::3])) == len(rows), "each tensor once"
     for first in range(0, len(rows), 12):
         some = rows[first:first + 12]
         launch(parents, "qd_reorder_states", *some, *(None, 0, 0) * (4 - len(some) // 3), ptr(parents), ptr(status), count)

@@ -568,7 +568,7 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
                               int* parents_out, void* tokens_out, void* scratch, int batch, int beams, int vocab, int candidates, int placed, void* stream) {
     QD_CHECK_ARG(logits && scores && scores_out && parents_out && tokens_out && (scratch || vocab <= kShortVocab) && batch > 0 && beams > 0 && vocab > 0 && candidates > 0);
     QD_CHECK_ARG((long long)beams * vocab >= candidates && (!finished || (eos >= 0 && eos < vocab)) && (!placed || candidates == beams));
-    QD_CHECK_ARG(((uintptr_t)scratch & 15u) == 0);
+    QD_CHECK_ARG(((uintptr_t)scratch & 15u) == 0 && vocab <= 0x7fffffff - 4096);           // (a chunk's places are 32-bit numbers)
     if (beams > kMostBeams || candidates > kMostBeams || (long long)batch * beams > 65535) return QD_ERR_UNSUPPORTED;
     SelectParams p;
     const long long rows = (long long)batch * beams;

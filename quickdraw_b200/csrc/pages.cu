@@ -245,8 +245,8 @@ QD_DEVINL void reserve_pages(const ReserveParams& p) {
             if (n < 0 || more < 0 || (long long)n + more > (long long)p.width * p.page) {
                 if (blockIdx.x == 0) atomicOr(p.status, QD_STATUS_BAD_ARG);
             } else if (more > 0) {
-                from = (n + p.page - 1) / p.page;
-                to = (n + more + p.page - 1) / p.page;
+                from = n ? (n - 1) / p.page + 1 : 0;
+                to = (n + more - 1) / p.page + 1;                           // (no sum passes the table's rows)
                 for (int j = from; j < to; ++j) need += read_now(p.table + (long long)b * p.width + j) < 0;
             }
         }

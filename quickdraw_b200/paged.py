@@ -35,7 +35,11 @@ def device_status(device) -> torch.Tensor:
     """The status word of a device that calls without a word of their own share."""
     word = _status.get(device)
     if word is None:
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        assert not capturing, "a graph's memory is not shared: call device_status(device) before the capture, or give a status"
         word = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()         # any stream may use it from now on
     return word
 
 
@@ -274,7 +278,11 @@ class PagedCache:
 class PagedBatchState:
     """The state of ``batch`` sequences for ``BatchDecode``, like ``BatchState``, with the attention layers' rows in a pool of ``pages``
     pages of ``page`` rows (default: enough for ``max_context`` rows of every sequence).  ``admit`` takes a prefilled prompt in, ``fork``
-    lets sequences go on as copies of others, ``free`` ends them."""
+    lets sequences go on as copies of others, ``free`` ends them.
+
+    A step appends a token to every place, to an empty one as well, which takes pages as any other does until it is freed again; where
+    a pool runs out of them ``cache.check`` says so.  ``admit`` may move a position past what a captured step (``graph_step``) has
+    counted to: ``BatchDecode.forget`` the state then."""
 
     def __init__(self, config, batch: int, max_context: int, device, pages: int | None = None, page: int = 64):
         one = DecodeState.allocate(config, 1, "meta")

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import decode_oracle as O
-from quickdraw_b200 import paged, synthetic
+from quickdraw_b200 import beam, paged, synthetic
 from tests import paged_plain as plain
 
 pytestmark = pytest.mark.gpu
@@ -283,6 +283,52 @@ def test_reserve(cuda_device):
     assert int(status) == 4 and (table >= 0).sum(1).tolist() == [3, 4, 1, 4]
     paged.reserve_pages(table, n, refs, 16, 40, status=status)         # one page is left, for the first
     assert int(status) == 12 and (table >= 0).sum(1).tolist() == [4, 4, 1, 4] and bool((refs == 1).all())
+
+
+def test_reserve_of_pages_as_long_as_numbers_go(cuda_device):
+    table, refs = torch.full((2, 1), -1, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    lengths, status = torch.tensor([0, 2 ** 31 - 4], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.reserve_pages(table, lengths, refs, 2 ** 31 - 1, 3, status=status)            # the second's page began long ago
+    assert table.tolist() == [[0], [-1]] and refs.tolist() == [1, 0, 0] and int(status) == 0
+    paged.reserve_pages(table, lengths, refs, 2 ** 31 - 1, 4, status=status)
+    assert table.tolist() == [[0], [-1]] and int(status) == paged.BAD_ARGUMENT
+
+
+def test_forks_and_reservations_from_a_graph(cuda_device):
+    def life(cache, state, parents, fork):
+        fork()
+        for _ in range(5):
+            parents.copy_(torch.roll(parents, 1))
+            fork()
+        return [cache.table.clone(), cache.lengths.clone(), cache.refs.clone(), state.clone(), cache.k.clone()]
+
+    results = []
+    for captured in (False, True):
+        cache = paged.PagedCache(2, 1, 64, 40, 8, 4, 64, "cuda")
+        cache.lengths.copy_(torch.tensor([13, 8, 0, 21], dtype=torch.int32))
+        counts = cache.lengths.clone()
+        cache.lengths.zero_()
+        cache.reserve(counts)
+        cache.lengths.copy_(counts)
+        cache.k.copy_(torch.arange(cache.k.numel(), device="cuda").view_as(cache.k) % 251)
+        state = torch.arange(4 * 48.0, device="cuda").view(4, 48).clone()
+        parents = torch.tensor([0, 0, 3, 1], dtype=torch.int32, device="cuda")
+
+        def step():
+            cache.reserve(3)
+            cache.lengths += 1
+            cache.fork(parents)
+            beam.reorder_states(state, parents, status=cache.status)
+
+        fork = step
+        if captured:
+            graph, other = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            with torch.cuda.graph(graph, stream=other):
+                step()
+            fork = graph.replay
+        results.append(life(cache, state, parents, fork))
+        assert cache.check() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
 def test_cache_through_its_life(cuda_device):

@@ -157,9 +157,21 @@ def test_reorder_passes_its_arguments_and_refuses(calls):
     for state in (torch.zeros(4, 4), torch.zeros(3, 4, 4).transpose(1, 2), torch.zeros(1, 4).expand(3, 4), torch.zeros(())):
         with pytest.raises(AssertionError):
             beam.reorder_states(on_gpu(state), parents, status=status)
+    twice = torch.zeros(3, 4)
+    with pytest.raises(AssertionError):
+        beam.reorder_states([on_gpu(twice), on_gpu(twice)], parents, status=status)
     with pytest.raises(AssertionError):
         beam.reorder_states(on_gpu(torch.zeros(3, 4)), on_gpu(torch.zeros(3, dtype=torch.long)), status=status)
     assert not calls
+
+
+def test_a_device_s_status_is_not_made_in_a_capture(monkeypatch):
+    monkeypatch.setattr(paged, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(AssertionError):
+        paged.device_status(torch.device("cuda", 0))
+    word = paged.device_status(torch.device("cpu"))
+    assert int(word) == 0 and paged.device_status(torch.device("cpu")) is word
 
 
 def test_search_refuses():
