@@ -3,7 +3,7 @@
 // A continuation of beam i by token v counts score[i] + x[i, v] - log sum_w exp x[i, w].  Within a beam the order is that of the logits, so a first
 // kernel takes, of each piece of a row, the largest logits, the maximum and the sum of exponentials, and a second one joins the pieces, adds up in 64
 // bits (sums of different beams lie next to one another) and merges the beams.
-#include "paged.cuh"
+#include "paged_tiles.cuh"
 
 namespace qd {
 namespace {
@@ -40,6 +40,24 @@ QD_DEVINL float exp_base2(float x) {             // (results below 2^-126 are ze
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two at a time, and the largest of three.
+QD_DEVINL float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+QD_DEVINL float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+QD_DEVINL float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Descending order of 32 keys, one a lane.
 QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 #pragma unroll
@@ -58,10 +76,12 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 // and again where more than a few threads have a key above it; it rises to the candidates-th of the list when that grows.
 // 32 x 8 rows of 151936, fp32 (156 MB): 36 us (4.3 TB/s), bf16 38: instructions, some eighteen a logit, half of them exponentials and sums.  A warp with a
 // list of its own took 52 (no barrier, but eight first chunks instead of one), lists of 256 keys 80; 256 threads 43.
-constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 48, kPartList = 3 * kMostBeams + 16;
+constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 32, kPartPending = 16, kPartSlack = 4;
+template <typename T, bool WHOLE> constexpr size_t part_ring() { return WHOLE ? 2 * kPartThreads * kPartEach * sizeof(T) : 0; }
 template <typename T, bool WHOLE>
-QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long long* part_list, unsigned long long* out) {
-    // part_list: kPartList, and what a chunk can add: kPartMany threads' keys, or those of K lanes of each warp.  out: the K largest keys, 0 behind the last
+QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long long* part_list, unsigned char* ring, unsigned long long* out) {
+    // part_list (part_bytes) has room for K + kPartSlack keys, for those of kPartPending threads and for what a chunk can add: kPartMany threads' keys, or
+    // those of K lanes of each warp.  ring: part_ring bytes on 16.  out: the K largest keys, 0 behind the last
     __shared__ unsigned long long bounds[kPartThreads / 32];
     __shared__ double2 sums[kPartThreads / 32];
     __shared__ int count;
@@ -70,13 +90,21 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
     // the thread's j-th logit of the chunk from `base`: four pieces of 16 bytes of fp32, two of bf16, or single ones
     constexpr int kRun = !WHOLE ? 1 : sizeof(T) == 4 ? 4 : 8;
     const auto place = [&](int base, int j) { return base + j / kRun * (kRun * kPartThreads) + tid * kRun + j % kRun; };
-    const auto fetch = [&](int base, float (&v)[kPartEach]) {
-        if (base + kPartThreads * kPartEach <= hi) {                            // (of all threads alike)
+    constexpr int kChunk = kPartThreads * kPartEach, kBytes = kChunk * (int)sizeof(T);
+    const uint32_t own = smem_u32(ring) + tid * 16;
+    const auto fetch = [&](int base, int slot) {
+        if (WHOLE && base <= hi - kChunk) {
+#pragma unroll
+            for (int j = 0; j < kPartEach / kRun; ++j) cp_async16(own + slot * kBytes + j * (kPartThreads * 16), x + place(base, j * kRun), 16);
+        }
+        cp_async_commit();
+    };
+    const auto take = [&](int base, int slot, float (&v)[kPartEach]) {
+        if (WHOLE && base <= hi - kChunk) {                                     // (of all threads alike)
 #pragma unroll
             for (int j = 0; j < kPartEach; j += kRun) {
-                if (!WHOLE) { v[j] = logit_of(x[place(base, j)]); continue; }
-                const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + place(base, j)));
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(own + slot * kBytes + j / kRun * (kPartThreads * 16)) : "memory");
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (sizeof(T) == 4) v[j + e] = __uint_as_float(w[e]);
@@ -102,28 +130,34 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             if (rank < K) into[rank] = key;
         }
     };
-    float top = -INFINITY, next[kPartEach];
+    float top = -INFINITY;
     double sum = 0.0;                  // of sums of sixteen: 32 bits would lose a ten-millionth with every few terms
     unsigned long long bound = 0;
     float least = -INFINITY;           // the bound's logit
-    fetch(lo, next);
+    int pending = 0;                   // threads that have put keys into the list since its length was looked at
+    fetch(lo, 0);
     __syncthreads();
-    for (int base = lo; base < hi; base += kPartThreads * kPartEach) {
+    for (int base = lo, slot = 0; base < hi; base += kChunk, slot ^= 1) {
         float v[kPartEach], most = -INFINITY;
+        cp_async_wait<0>();
+        take(base, slot, v);
+        fetch(base + kChunk, slot ^ 1);
 #pragma unroll
-        for (int j = 0; j < kPartEach; ++j) { v[j] = next[j]; most = fmaxf(most, v[j]); }
-        if (base + kPartThreads * kPartEach < hi) fetch(base + kPartThreads * kPartEach, next);
+        for (int j = 0; j < kPartEach; j += 2) most = max3(most, v[j], v[j + 1]);
         // (terms of up to e^2 lose nothing, and few chunks rescale)
         if (most > top + 2.f) { sum *= (double)exp_base2((top - most) * 1.4426950408889634f); top = most; }
         const float shift = top == -INFINITY ? 0.f : top;
-        float e[kPartEach];
+        float2 e[kPartEach / 2];
 #pragma unroll
-        for (int j = 0; j < kPartEach; ++j) e[j] = exp_base2((v[j] - shift) * 1.4426950408889634f);      // (NaN and infinity go on)
+        for (int j = 0; j < kPartEach / 2; ++j) {                               // (NaN and infinity go on)
+            e[j] = mul2(add2(make_float2(v[2 * j], v[2 * j + 1]), make_float2(-shift, -shift)), make_float2(1.4426950408889634f, 1.4426950408889634f));
+            e[j] = make_float2(exp_base2(e[j].x), exp_base2(e[j].y));
+        }
 #pragma unroll
-        for (int d = kPartEach / 2; d > 0; d >>= 1)
+        for (int d = kPartEach / 4; d > 0; d >>= 1)
 #pragma unroll
-            for (int j = 0; j < d; ++j) e[j] += e[j + d];
-        sum += (double)e[0];
+            for (int j = 0; j < d; ++j) e[j] = add2(e[j], e[j + d]);
+        sum += (double)(e[0].x + e[0].y);
         const bool hit = most >= least;
         const int above = __syncthreads_count(hit);
         if (above == 0) continue;
@@ -140,16 +174,23 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             if (bound) least = key_logit(bound);
         }
         if (hit) {
+            unsigned mask = 0;
 #pragma unroll
-            for (int j = 0; j < kPartEach; ++j)
-                if (v[j] >= least) {
-                    const unsigned long long key = key_of(j);
-                    if (key > bound) part_list[atomicAdd(&count, 1)] = key;
-                }
+            for (int j = 0; j < kPartEach; ++j) mask |= v[j] >= least ? 1u << j : 0u;
+            for (; mask; mask &= mask - 1u) {
+                const int j = __ffs(mask) - 1, at = place(base, j);
+                if (at >= hi) break;
+                const T* from = WHOLE && base <= hi - kChunk ? (const T*)(ring + tid * 16 + slot * kBytes + j / kRun * (kPartThreads * 16)) + j % kRun : x + at;
+                const unsigned long long key = logit_key(logit_of(*from), at);
+                if (key > bound) part_list[atomicAdd(&count, 1)] = key;
+            }
         }
+        pending += above;
+        if (pending <= kPartPending) continue;
+        pending = 0;
         __syncthreads();
         const int n = count;
-        if (n > 3 * K + 16) {                                                   // (a thread counts n keys: often and few is less than seldom and many)
+        if (n > K + kPartSlack) {                                                   // (a thread counts n keys: often and few is less than seldom and many)
             keep(out, n);                                                       // (the results' place serves as scratch)
             __syncthreads();
             if (tid < K) part_list[tid] = out[tid];
@@ -159,6 +200,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             __syncthreads();
         }
     }
+    __syncthreads();
     const int n = count;
     for (int k = n + tid; k < K; k += kPartThreads) out[k] = 0;
     keep(out, n);
@@ -180,7 +222,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
     return make_double2((double)all, total);
 }
 static size_t part_bytes(int candidates) {
-    return sizeof(unsigned long long) * (kPartList + kPartEach * (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates));
+    return sizeof(unsigned long long) * (candidates + kPartSlack + kPartEach * (kPartPending + (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates)));
 }
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
@@ -190,7 +232,7 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     if (p.finished && p.finished[row]) return;
     const int lo = (int)((long long)each * split / p.splits) * 8, hi = split + 1 == p.splits ? p.vocab : (int)((long long)each * (split + 1) / p.splits) * 8;
     const long long at = (long long)row * p.splits + split;
-    const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, lo, hi, p.candidates, select_list, p.keys + at * p.candidates);
+    const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, lo, hi, p.candidates, select_list + part_ring<T, WHOLE>() / 8, (unsigned char*)select_list, p.keys + at * p.candidates);
     if (threadIdx.x == 0) p.sums[at] = sum;
 }
 
@@ -426,7 +468,7 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
         const int beam = block + i * kMergeBlocks;
         if (finished(beam)) continue;
         const long long row = (long long)group * p.beams + beam;
-        const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, 0, p.vocab, K, list, keys[i]);
+        const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, 0, p.vocab, K, list + part_ring<T, WHOLE>() / 8, (unsigned char*)list, keys[i]);
         if (threadIdx.x == 0) sums[i] = sum;
         __syncthreads();
     }
@@ -547,6 +589,14 @@ int reorder_launch(const ReorderParams& p, dim3 grid, size_t smem, cudaStream_t 
     return qd_launch(reorder_kernel<U>, grid, dim3(kReorderThreads), smem, stream, 3, p);
 }
 
+template <typename T, bool WHOLE>
+int short_launch(const SelectParams& p, size_t part, cudaStream_t stream) {
+    const size_t smem = part + part_ring<T, WHOLE>() + (p.beams * p.candidates * 12 + 15) / 16 * 16;              // at most 47 KB, beside what is declared
+    static bool raised[kDevices];
+    if (smem > 40 * 1024 && !raise_smem(select_short_kernel<T, WHOLE>, 48 * 1024, raised)) return QD_ERR_LAUNCH;
+    return qd_launch(select_short_kernel<T, WHOLE>, dim3(p.batch * kMergeBlocks), dim3(kMergeThreads), smem, stream, 3, p);
+}
+
 int splits_of(long long rows, int vocab) {
     const long long want = device_blocks() * 8ll / rows, most = vocab / 2048;
     const long long s = want < most ? want : most;
@@ -583,19 +633,14 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
     const size_t part = part_bytes(candidates);
     const dim3 grid(p.splits, (unsigned)rows);
     const cudaStream_t on = (cudaStream_t)stream;
-    if (vocab <= kShortVocab) {
-        const size_t both = part + (beams * candidates * 12 + 15) / 16 * 16;          // at most 30 KB
-        const dim3 clusters(batch * kMergeBlocks);
-        if (whole) return is_fp32 ? qd_launch(select_short_kernel<float, true>, clusters, dim3(kMergeThreads), both, on, 3, p)
-                                  : qd_launch(select_short_kernel<bf16, true>, clusters, dim3(kMergeThreads), both, on, 3, p);
-        return is_fp32 ? qd_launch(select_short_kernel<float, false>, clusters, dim3(kMergeThreads), both, on, 3, p)
-                       : qd_launch(select_short_kernel<bf16, false>, clusters, dim3(kMergeThreads), both, on, 3, p);
-    }
+    if (vocab <= kShortVocab)
+        return whole ? is_fp32 ? short_launch<float, true>(p, part, on) : short_launch<bf16, true>(p, part, on)
+                     : is_fp32 ? short_launch<float, false>(p, part, on) : short_launch<bf16, false>(p, part, on);
     int code;
-    if (whole) code = is_fp32 ? qd_launch(select_part_kernel<float, true>, grid, dim3(kPartThreads), part, on, 3, p)
-                              : qd_launch(select_part_kernel<bf16, true>, grid, dim3(kPartThreads), part, on, 3, p);
-    else code = is_fp32 ? qd_launch(select_part_kernel<float, false>, grid, dim3(kPartThreads), part, on, 3, p)
-                        : qd_launch(select_part_kernel<bf16, false>, grid, dim3(kPartThreads), part, on, 3, p);
+    if (whole) code = is_fp32 ? qd_launch(select_part_kernel<float, true>, grid, dim3(kPartThreads), part + part_ring<float, true>(), on, 3, p)
+                              : qd_launch(select_part_kernel<bf16, true>, grid, dim3(kPartThreads), part + part_ring<bf16, true>(), on, 3, p);
+    else code = is_fp32 ? qd_launch(select_part_kernel<float, false>, grid, dim3(kPartThreads), part + part_ring<float, false>(), on, 3, p)
+                        : qd_launch(select_part_kernel<bf16, false>, grid, dim3(kPartThreads), part + part_ring<bf16, false>(), on, 3, p);
     if (code != QD_OK) return code;
     const int lists = p.splits < candidates ? p.splits : candidates;
     const size_t smem = 8ull * (beams * candidates + (beams * candidates + 1) / 2 + (size_t)(kMergeThreads / 32) * lists * candidates);       // at most 44 KB
