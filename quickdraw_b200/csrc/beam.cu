@@ -72,17 +72,18 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 }
 
 // A block per piece of a row, one pass: sixteen logits a thread at a time, their maximum and sum of exponentials, and a list of the keys above a bound that
-// `candidates` keys seen so far reach.  The bound comes from the first chunk (of each warp's 32 largest keys the candidates-th, of these the largest),
-// and again where more than a few threads have a key above it; it rises to the candidates-th of the list when that grows.
-// 32 x 8 rows of 151936, fp32 (156 MB): 36 us (4.3 TB/s), bf16 38: instructions, some eighteen a logit, half of them exponentials and sums.  A warp with a
-// list of its own took 52 (no barrier, but eight first chunks instead of one), lists of 256 keys 80; 256 threads 43.
+// `candidates` keys seen so far reach.  The bound comes from the lanes' largest keys of the first chunk, and again where more than a few threads have a key
+// above it; it rises to the candidates-th of the list when that grows.  32 x 8 rows of 151936 with the merge: 39.5 us fp32 (156 MB, of it 35 us with no
+// keys and no exponentials to take), 37.6 bf16; 43 and 46 with the next chunk in registers (fewer blocks an SM) and a second barrier in every chunk that
+// has a key.  Two chunks ahead took 42 (fewer blocks), a warp with a list of its own ten more (eight first chunks instead of one), 256 threads seven more.
+// 4 x 32 rows: 65 us, 98 with a first bound from each warp alone (a fifth of the chunk is above it).
 constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 32, kPartPending = 16, kPartSlack = 4;
 template <typename T, bool WHOLE> constexpr size_t part_ring() { return WHOLE ? 2 * kPartThreads * kPartEach * sizeof(T) : 0; }
 template <typename T, bool WHOLE>
 QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long long* part_list, unsigned char* ring, unsigned long long* out) {
     // part_list (part_bytes) has room for K + kPartSlack keys, for those of kPartPending threads and for what a chunk can add: kPartMany threads' keys, or
     // those of K lanes of each warp.  ring: part_ring bytes on 16.  out: the K largest keys, 0 behind the last
-    __shared__ unsigned long long bounds[kPartThreads / 32];
+    __shared__ unsigned long long bounds[2 * (kPartThreads / 32)];
     __shared__ double2 sums[kPartThreads / 32];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -116,7 +117,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             for (int j = 0; j < kPartEach; ++j) v[j] = place(base, j) < hi ? logit_of(x[place(base, j)]) : -INFINITY;
         }
     };
-    // the `K` largest of the list, in order: a thread counts for its keys how many are larger
+    // the K largest of the list, in order: a thread counts for its keys how many are larger
     const auto keep = [&](unsigned long long* into, int n) {
         for (int i = tid; i < n; i += kPartThreads) {
             const unsigned long long key = part_list[i];
@@ -166,11 +167,18 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             unsigned long long mine = 0;
 #pragma unroll
             for (int j = 0; j < kPartEach; ++j) mine = key_of(j) > mine ? key_of(j) : mine;
-            const unsigned long long kth = __shfl_sync(0xffffffffu, warp_sorted(mine, lane), K - 1);
-            if (lane == 0) bounds[warp] = kth ? kth - 1 : 0;
+            // K keys are as large as a warp's K-th, and as the least of all warps' shares of K
+            constexpr int kAll = kPartThreads / 32;
+            const unsigned long long sorted = warp_sorted(mine, lane), kth = __shfl_sync(0xffffffffu, sorted, K - 1), share = __shfl_sync(0xffffffffu, sorted, (K - 1) / kAll);
+            if (lane == 0) { bounds[warp] = kth; bounds[kAll + warp] = share; }
             __syncthreads();
+            unsigned long long least_share = bounds[kAll];
 #pragma unroll
-            for (int w = 0; w < kPartThreads / 32; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+            for (int w = 0; w < kAll; ++w) {
+                bound = bounds[w] > bound ? bounds[w] - 1 : bound;
+                least_share = bounds[kAll + w] < least_share ? bounds[kAll + w] : least_share;
+            }
+            bound = least_share > bound ? least_share - 1 : bound;
             if (bound) least = key_logit(bound);
         }
         if (hit) {
@@ -419,7 +427,8 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
     int n = 0;
     if (there && !finished) {
         const unsigned long long* keys = p.keys + row * p.splits * K;
-        const unsigned long long head = lane < p.splits ? keys[lane * K] : 0;
+        const int deep = (K + p.splits - 1) / p.splits, pieces = (K + deep - 1) / deep;
+        const unsigned long long head = lane < p.splits ? keys[lane * K + deep - 1] : 0;
         const double2 s = lane < p.splits ? p.sums[row * p.splits + lane] : make_double2(-INFINITY, 0.0);
         top = warp_max((float)s.x);
         const bool odd = __any_sync(0xffffffffu, lane < p.splits && (s.x != s.x || s.y != s.y));
@@ -428,8 +437,8 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         lse = (double)top + log(sum);
         counts = counts && !odd && isfinite(lse);
-        // no piece but those with one of the K largest heads has any of the K largest keys; of these, the keys that are as large as the K-th head
-        const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), K - 1);
+        // `pieces` of them have `deep` keys each, K or more in all, that are no smaller than the largest bound for which that is so: keys below it are out
+        const unsigned long long bound = __shfl_sync(0xffffffffu, warp_sorted(head, lane), pieces - 1);
         for (int k = lane; counts && k < (p.splits * K + 31) / 32 * 32; k += 32) {
             const unsigned long long key = k < p.splits * K ? keys[k] : 0;
             const bool in = key && key >= bound;
