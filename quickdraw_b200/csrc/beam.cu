@@ -78,8 +78,8 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 // has a key.  Two chunks ahead took 42 (fewer blocks), a warp with a list of its own ten more (eight first chunks instead of one), 256 threads seven more.
 // 4 x 32 rows: 65 us, 98 with a first bound from each warp alone (a fifth of the chunk is above it).
 constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 32, kPartPending = 16, kPartSlack = 4;
-template <typename T, bool WHOLE> constexpr size_t part_ring() { return WHOLE ? 2 * kPartThreads * kPartEach * sizeof(T) : 0; }
-template <typename T, bool WHOLE>
+template <typename T> constexpr size_t part_ring() { return 2 * kPartThreads * kPartEach * sizeof(T); }
+template <typename T>
 QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long long* part_list, unsigned char* ring, unsigned long long* out) {
     // part_list (part_bytes) has room for K + kPartSlack keys, for those of kPartPending threads and for what a chunk can add: kPartMany threads' keys, or
     // those of K lanes of each warp.  ring: part_ring bytes on 16.  out: the K largest keys, 0 behind the last
@@ -88,20 +88,23 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) count = 0;
-    // the thread's j-th logit of the chunk from `base`: four pieces of 16 bytes of fp32, two of bf16, or single ones
-    constexpr int kRun = !WHOLE ? 1 : sizeof(T) == 4 ? 4 : 8;
+    // the thread's j-th logit of the chunk from `base`: four pieces of 16 bytes of fp32, two of bf16; the first chunk begins on a piece in front of `lo`
+    constexpr int kRun = sizeof(T) == 4 ? 4 : 8;
     const auto place = [&](int base, int j) { return base + j / kRun * (kRun * kPartThreads) + tid * kRun + j % kRun; };
     constexpr int kChunk = kPartThreads * kPartEach, kBytes = kChunk * (int)sizeof(T);
     const uint32_t own = smem_u32(ring) + tid * 16;
+    const int start = lo - (int)((reinterpret_cast<uintptr_t>(x + lo) & 15u) / sizeof(T));
+    const auto whole = [&](int base) { return base >= lo && base <= hi - kChunk; };             // (of all threads alike)
+    const auto is_there = [&](int at) { return at >= lo && at < hi; };
     const auto fetch = [&](int base, int slot) {
-        if (WHOLE && base <= hi - kChunk) {
+        if (whole(base)) {
 #pragma unroll
             for (int j = 0; j < kPartEach / kRun; ++j) cp_async16(own + slot * kBytes + j * (kPartThreads * 16), x + place(base, j * kRun), 16);
         }
         cp_async_commit();
     };
     const auto take = [&](int base, int slot, float (&v)[kPartEach]) {
-        if (WHOLE && base <= hi - kChunk) {                                     // (of all threads alike)
+        if (whole(base)) {
 #pragma unroll
             for (int j = 0; j < kPartEach; j += kRun) {
                 uint32_t w[4];
@@ -114,7 +117,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < kPartEach; ++j) v[j] = place(base, j) < hi ? logit_of(x[place(base, j)]) : -INFINITY;
+            for (int j = 0; j < kPartEach; ++j) v[j] = is_there(place(base, j)) ? logit_of(x[place(base, j)]) : -INFINITY;
         }
     };
     // the K largest of the list, in order: a thread counts for its keys how many are larger
@@ -136,9 +139,9 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
     unsigned long long bound = 0;
     float least = -INFINITY;           // the bound's logit
     int pending = 0;                   // threads that have put keys into the list since its length was looked at
-    fetch(lo, 0);
+    fetch(start, 0);
     __syncthreads();
-    for (int base = lo, slot = 0; base < hi; base += kChunk, slot ^= 1) {
+    for (int base = start, slot = 0; base < hi; base += kChunk, slot ^= 1) {
         float v[kPartEach], most = -INFINITY;
         cp_async_wait<0>();
         take(base, slot, v);
@@ -162,7 +165,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
         const bool hit = most >= least;
         const int above = __syncthreads_count(hit);
         if (above == 0) continue;
-        const auto key_of = [&](int j) { return place(base, j) < hi ? logit_key(v[j], place(base, j)) : 0; };       // places behind the end: none
+        const auto key_of = [&](int j) { return is_there(place(base, j)) ? logit_key(v[j], place(base, j)) : 0; };       // other places: none
         if (above > kPartMany) {
             unsigned long long mine = 0;
 #pragma unroll
@@ -187,8 +190,8 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
             for (int j = 0; j < kPartEach; ++j) mask |= v[j] >= least ? 1u << j : 0u;
             for (; mask; mask &= mask - 1u) {
                 const int j = __ffs(mask) - 1, at = place(base, j);
-                if (at >= hi) break;
-                const T* from = WHOLE && base <= hi - kChunk ? (const T*)(ring + tid * 16 + slot * kBytes + j / kRun * (kPartThreads * 16)) + j % kRun : x + at;
+                if (!is_there(at)) continue;
+                const T* from = whole(base) ? (const T*)(ring + tid * 16 + slot * kBytes + j / kRun * (kPartThreads * 16)) + j % kRun : x + at;
                 const unsigned long long key = logit_key(logit_of(*from), at);
                 if (key > bound) part_list[atomicAdd(&count, 1)] = key;
             }
@@ -232,7 +235,7 @@ QD_DEVINL double2 part_of_row(const T* x, int lo, int hi, int K, unsigned long l
 static size_t part_bytes(int candidates) {
     return sizeof(unsigned long long) * (candidates + kPartSlack + kPartEach * (kPartPending + (kPartMany > kPartThreads / 32 * candidates ? kPartMany : kPartThreads / 32 * candidates)));
 }
-template <typename T, bool WHOLE>
+template <typename T>
 __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectParams p) {
     chain_enter();
     extern __shared__ __align__(16) unsigned long long select_list[];
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(kPartThreads) select_part_kernel(const SelectP
     if (p.finished && p.finished[row]) return;
     const int lo = (int)((long long)each * split / p.splits) * 8, hi = split + 1 == p.splits ? p.vocab : (int)((long long)each * (split + 1) / p.splits) * 8;
     const long long at = (long long)row * p.splits + split;
-    const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, lo, hi, p.candidates, select_list + part_ring<T, WHOLE>() / 8, (unsigned char*)select_list, p.keys + at * p.candidates);
+    const double2 sum = part_of_row<T>((const T*)p.logits + row * p.row_stride, lo, hi, p.candidates, select_list + part_ring<T>() / 8, (unsigned char*)select_list, p.keys + at * p.candidates);
     if (threadIdx.x == 0) p.sums[at] = sum;
 }
 
@@ -458,7 +461,7 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
 // the host 5 us with its scratch; on the device 500 tokens of 16 x 16 beams take 17.9 instead of 17.7 us, 4096 of 1 x 4 9.9 instead of 10.4, but of 16 x 16
 // 27 instead of 19).
 constexpr int kShortVocab = kPartThreads * kPartEach;
-template <typename T, bool WHOLE>
+template <typename T>
 __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThreads) select_short_kernel(const SelectParams p) {
     static_assert(kMergeThreads == kPartThreads, "a block is both");
     chain_enter();
@@ -477,7 +480,7 @@ __global__ void __cluster_dims__(kMergeBlocks, 1, 1) __launch_bounds__(kMergeThr
         const int beam = block + i * kMergeBlocks;
         if (finished(beam)) continue;
         const long long row = (long long)group * p.beams + beam;
-        const double2 sum = part_of_row<T, WHOLE>((const T*)p.logits + row * p.row_stride, 0, p.vocab, K, list + part_ring<T, WHOLE>() / 8, (unsigned char*)list, keys[i]);
+        const double2 sum = part_of_row<T>((const T*)p.logits + row * p.row_stride, 0, p.vocab, K, list + part_ring<T>() / 8, (unsigned char*)list, keys[i]);
         if (threadIdx.x == 0) sums[i] = sum;
         __syncthreads();
     }
@@ -598,12 +601,12 @@ int reorder_launch(const ReorderParams& p, dim3 grid, size_t smem, cudaStream_t 
     return qd_launch(reorder_kernel<U>, grid, dim3(kReorderThreads), smem, stream, 3, p);
 }
 
-template <typename T, bool WHOLE>
+template <typename T>
 int short_launch(const SelectParams& p, size_t part, cudaStream_t stream) {
-    const size_t smem = part + part_ring<T, WHOLE>() + (p.beams * p.candidates * 12 + 15) / 16 * 16;              // at most 47 KB, beside what is declared
+    const size_t smem = part + part_ring<T>() + (p.beams * p.candidates * 12 + 15) / 16 * 16;              // at most 47 KB, beside what is declared
     static bool raised[kDevices];
-    if (smem > 40 * 1024 && !raise_smem(select_short_kernel<T, WHOLE>, 48 * 1024, raised)) return QD_ERR_LAUNCH;
-    return qd_launch(select_short_kernel<T, WHOLE>, dim3(p.batch * kMergeBlocks), dim3(kMergeThreads), smem, stream, 3, p);
+    if (smem > 40 * 1024 && !raise_smem(select_short_kernel<T>, 48 * 1024, raised)) return QD_ERR_LAUNCH;
+    return qd_launch(select_short_kernel<T>, dim3(p.batch * kMergeBlocks), dim3(kMergeThreads), smem, stream, 3, p);
 }
 
 int splits_of(long long rows, int vocab) {
@@ -637,19 +640,13 @@ extern "C" int qd_beam_select(const void* logits, long long row_stride, int is_f
     p.keys = (unsigned long long*)(p.sums + rows * p.splits);
     p.scores_out = scores_out; p.parents_out = parents_out; p.tokens_out = (long long*)tokens_out;
     p.batch = batch; p.beams = beams; p.vocab = vocab; p.candidates = candidates; p.eos = eos; p.placed = placed; p.fp32 = is_fp32;
-    const int size = is_fp32 ? 4 : 2;
-    const bool whole = !(((uintptr_t)logits | (uintptr_t)(row_stride * size)) & 15u);
+    if ((uintptr_t)logits % (is_fp32 ? 4 : 2)) return QD_ERR_UNSUPPORTED;
     const size_t part = part_bytes(candidates);
     const dim3 grid(p.splits, (unsigned)rows);
     const cudaStream_t on = (cudaStream_t)stream;
-    if (vocab <= kShortVocab)
-        return whole ? is_fp32 ? short_launch<float, true>(p, part, on) : short_launch<bf16, true>(p, part, on)
-                     : is_fp32 ? short_launch<float, false>(p, part, on) : short_launch<bf16, false>(p, part, on);
-    int code;
-    if (whole) code = is_fp32 ? qd_launch(select_part_kernel<float, true>, grid, dim3(kPartThreads), part + part_ring<float, true>(), on, 3, p)
-                              : qd_launch(select_part_kernel<bf16, true>, grid, dim3(kPartThreads), part + part_ring<bf16, true>(), on, 3, p);
-    else code = is_fp32 ? qd_launch(select_part_kernel<float, false>, grid, dim3(kPartThreads), part + part_ring<float, false>(), on, 3, p)
-                        : qd_launch(select_part_kernel<bf16, false>, grid, dim3(kPartThreads), part + part_ring<bf16, false>(), on, 3, p);
+    if (vocab <= kShortVocab) return is_fp32 ? short_launch<float>(p, part, on) : short_launch<bf16>(p, part, on);
+    const int code = is_fp32 ? qd_launch(select_part_kernel<float>, grid, dim3(kPartThreads), part + part_ring<float>(), on, 3, p)
+                             : qd_launch(select_part_kernel<bf16>, grid, dim3(kPartThreads), part + part_ring<bf16>(), on, 3, p);
     if (code != QD_OK) return code;
     const int lists = p.splits < candidates ? p.splits : candidates;
     const size_t smem = 8ull * (beams * candidates + (beams * candidates + 1) / 2 + (size_t)(kMergeThreads / 32) * lists * candidates);       // at most 44 KB
