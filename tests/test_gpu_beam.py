@@ -112,6 +112,32 @@ def test_rows_of_a_larger_matrix_and_a_graph(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [1, 7, 2041, 2047, 2048, 2049, 4100, 6151])
+def test_rows_that_begin_anywhere(cuda_device, vocab, dtype):
+    """Between the rows lies what would spoil them."""
+    g = torch.Generator().manual_seed(vocab)
+    for first in range(9):
+        whole = torch.full((6, vocab + 17 - first), math.nan, dtype=dtype, device="cuda")
+        whole[:, first:first + vocab] = (torch.randn((6, vocab), generator=g) * 3).to(dtype).cuda()
+        logits = whole[:, first:first + vocab].unflatten(0, (2, 3))
+        scores = torch.randn((2, 3), generator=g).cuda()
+        same(beam.beam_select(logits, scores), logits, scores)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("candidates", [1, 8, 32])
+@pytest.mark.parametrize("order", ["up", "down", "steps", "one in front"])
+def test_rows_in_order(cuda_device, order, candidates, dtype):
+    """Every chunk above those before it, below them, of equal logits, or below one."""
+    vocab = 30011
+    row = {"up": torch.linspace(-9, 9, vocab), "down": torch.linspace(9, -9, vocab), "steps": torch.arange(vocab).div(2048, rounding_mode="floor") * 0.5,
+           "one in front": torch.cat((torch.tensor([5.0]), torch.zeros(vocab - 1)))}[order]
+    logits = torch.stack((row, row.roll(77), row.flip(0))).view(1, 3, vocab).to(dtype).cuda()
+    scores = torch.tensor([[0.0, -0.3, -0.7]], device="cuda")
+    same(beam.beam_select(logits, scores, candidates=candidates), logits, scores, candidates=candidates)
+
+
 @pytest.mark.parametrize("count,parents", [(1, [0]), (2, [1, 0]), (5, [4, 4, 4, 4, 4]), (4, [1, 2, 3, 0]), (6, [-1, 0, 0, 3, -1, 4]), (3, [0, 1, 2]), (3, [-1, -1, -1])])
 def test_reorder(cuda_device, count, parents):
     shapes = [((3, 8, 16), F32), ((5,), BF16), ((700, 33), BF16), ((7,), torch.uint8), ((1, 1), F32), ((0,), F32)]
