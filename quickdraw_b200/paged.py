@@ -128,12 +128,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 def _check_tables(table, refs, device):
-    assert table.ndim == 2 and _is_ids(table, device, *table.shape) and refs.ndim == 1 and _is_ids(refs, device, *refs.shape)
-    assert 0 < table.numel() < 2 ** 31 - 8192 and refs.numel() > 0
-
-
-def _scratch(table, refs):
-    return table.new_empty(scratch_size(table.get_device(), "qd_pages_scratch_words", *table.shape, refs.numel()))
+    """A table [sequences, width] and counts [pages] on `device`; their sizes, and scratch for them."""
+    assert table.dtype is torch.int32 and refs.dtype is torch.int32 and table.get_device() == device and refs.get_device() == device
+    assert table.ndim == 2 and refs.ndim == 1 and table.is_contiguous() and refs.is_contiguous()
+    (count, width), (pages,) = table.shape, refs.shape
+    assert 0 < count * width < 2 ** 31 - 8192 and pages > 0
+    return count, width, pages, table.new_empty(scratch_size(device, "qd_pages_scratch_words", count, width, pages))
 
 
 def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, *,
@@ -146,15 +146,14 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     A parent that is no sequence leaves its child as it is, and a child for which no page is left ends where its full pages do; both
     set bits of ``status`` (int32 [1]; a word shared by the device, ``device_status``, if not given)."""
     page_bytes, layer_bytes, row_bytes, layers = _check_pools(k_pages, v_pages)
-    device, (pages, _, page, _, _) = k_pages.get_device(), k_pages.shape
-    _check_tables(table, refs, device)
-    count, width = table.shape
-    assert _is_ids(lengths, device, count) and _is_ids(parents, device, count) and refs.numel() == pages and width * page < 2 ** 31
+    device, (in_pool, _, page, _, _) = k_pages.get_device(), k_pages.shape
+    count, width, pages, scratch = _check_tables(table, refs, device)
+    assert _is_ids(lengths, device, count) and _is_ids(parents, device, count) and pages == in_pool and width * page < 2 ** 31
     status = device_status(k_pages.device) if status is None else status
     assert _is_ids(status, device, 1)
     table_out, lengths_out, refs_out = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refs)
     launch(k_pages, "qd_pages_fork", ptr(k_pages), ptr(v_pages), page_bytes, layer_bytes, row_bytes, layers, ptr(table), ptr(lengths), ptr(refs),
-           ptr(parents), ptr(table_out), ptr(lengths_out), ptr(refs_out), ptr(_scratch(table, refs)), ptr(status), count, width, pages, page)
+           ptr(parents), ptr(table_out), ptr(lengths_out), ptr(refs_out), ptr(scratch), ptr(status), count, width, pages, page)
     return table_out, lengths_out, refs_out
 
 
@@ -163,12 +162,12 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     new (table, refs) and the number of pages in use (0-d int32, on the device).  Pages that are not used any more keep what they
     hold."""
     page_bytes, layer_bytes, row_bytes, layers = _check_pools(k_pages, v_pages)
-    device, (pages, _, page, _, _) = k_pages.get_device(), k_pages.shape
-    _check_tables(table, refs, device)
-    assert refs.numel() == pages
+    in_pool, _, page, _, _ = k_pages.shape
+    count, width, pages, scratch = _check_tables(table, refs, k_pages.get_device())
+    assert pages == in_pool
     table_out, refs_out, used = torch.empty_like(table), torch.empty_like(refs), table.new_empty(())
     launch(k_pages, "qd_pages_compact", ptr(k_pages), ptr(v_pages), page_bytes, layer_bytes, row_bytes, layers, ptr(table), ptr(refs), ptr(table_out),
-           ptr(refs_out), ptr(used), ptr(_scratch(table, refs)), *table.shape, pages, page)
+           ptr(refs_out), ptr(used), ptr(scratch), count, width, pages, page)
     return table_out, refs_out, used
 
 
@@ -177,15 +176,14 @@ def reserve_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor
     ``refs``: the lowest free ones, in the order of the sequences.  Rows past the table and an empty pool set bits of ``status``."""
     assert table.is_cuda
     device = table.get_device()
-    _check_tables(table, refs, device)
-    count, width = table.shape
+    count, width, pages, scratch = _check_tables(table, refs, device)
     each = isinstance(counts, torch.Tensor)
     assert _is_ids(lengths, device, count) and page > 0 and width * page < 2 ** 31
     assert _is_ids(counts, device, count) if each else 0 <= counts < 2 ** 31, "rows to come: a number, or int32 for every sequence"
     status = device_status(table.device) if status is None else status
     assert _is_ids(status, device, 1)
     launch(table, "qd_pages_reserve", ptr(table), ptr(lengths), ptr(refs), ptr(counts) if each else None, 0 if each else int(counts),
-           ptr(_scratch(table, refs)), ptr(status), count, width, refs.numel(), page)
+           ptr(scratch), ptr(status), count, width, pages, page)
 
 
 class PagedCache:
