@@ -47,8 +47,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
 
 
 def reorder_states(states, parents: torch.Tensor, *, status: torch.Tensor | None = None) -> None:
-    """``state[b] = old state[parents[b]]`` in place, for tensors [sequences, ...] (rows contiguous, any distance apart): -1 is a row of
-    zeros, a row that is its own parent is not touched, one whose parent is no row neither (a bit of ``status``)."""
+    """``state[b] = old state[parents[b]]`` in place, for tensors [sequences, ...] that do not overlap (rows contiguous, any distance apart): -1 is
+    a row of zeros, a row that is its own parent is not touched, one whose parent is no row neither (a bit of ``status``)."""
     states = [states] if isinstance(states, torch.Tensor) else list(states)
     assert parents.is_cuda and parents.ndim == 1 and _is_ids(parents, parents.get_device(), *parents.shape) and parents.numel() > 0
     device, count = parents.get_device(), parents.numel()

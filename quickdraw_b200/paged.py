@@ -220,8 +220,8 @@ class PagedCache:
 
     def free(self, sequences) -> None:
         """The sequences of these numbers end."""
-        assert all(0 <= b < self.sequences for b in sequences), "no such sequence"
         ends = set(sequences)
+        assert all(0 <= b < self.sequences for b in ends), "no such sequence"
         self.fork(torch.tensor([-1 if b in ends else b for b in range(self.sequences)], dtype=torch.int32).to(self.table.device, non_blocking=True))
 
     def compact(self) -> torch.Tensor:
@@ -323,8 +323,8 @@ class PagedBatchState:
 
     def free(self, sequences) -> None:
         """The sequences of these numbers end; their places are empty."""
-        assert all(0 <= b < self.batch for b in sequences), "no such sequence"
         ends = set(sequences)
+        assert all(0 <= b < self.batch for b in ends), "no such sequence"
         self.fork(torch.tensor([-1 if b in ends else b for b in range(self.batch)], dtype=torch.int32).to(self.cache.table.device, non_blocking=True))
 
     def memory_bytes(self) -> int:

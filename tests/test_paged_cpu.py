@@ -110,6 +110,17 @@ def test_reserves_refuse(calls):
     assert not calls
 
 
+@pytest.mark.parametrize("several", [list, iter, set, range])
+def test_sequences_end_by_any_row_of_numbers(monkeypatch, several):
+    cache = paged.PagedCache(1, 1, 8, 4, 4, 3, 8, "cpu")
+    seen = []
+    monkeypatch.setattr(cache, "fork", lambda parents: seen.append(parents.tolist()))
+    cache.free(range(1, 3) if several is range else several([1, 2]))
+    assert seen == [[0, -1, -1]]
+    with pytest.raises(AssertionError):
+        cache.free(iter([0, 3]))
+
+
 def test_cache_of_no_size_is_refused():
     for sizes in ((0, 2, 64, 4, 16, 2, 100), (1, 2, 64, 0, 16, 2, 100), (1, 2, 64, 4, 0, 2, 100), (1, 2, 64, 4, 16, 0, 100), (1, 2, 64, 4, 16, 2, 0)):
         with pytest.raises(AssertionError):
