@@ -30,6 +30,26 @@ static inline bool raise_smem(void (*kernel)(KArgs...), size_t bytes, bool (&rai
     return raised[dev];
 }
 
+// Two numbers in one instruction.
+QD_DEVINL float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+QD_DEVINL float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+QD_DEVINL float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // A sequence is cut into parts by its own length, the number of (sequence, key/value head, chunk of heads) triples and that of workers alone, so that
 // its result does not depend on its neighbours: as if all of the batch were as long, so that they fill some rounds of workers in least time (a part
 // costs `kPagedFixed` units beside its own: its state is written, read and joined); of cuts that are within 1 / 16 of it the finest, because beside

@@ -15,7 +15,8 @@ template <int D, int HEADS> struct PagedFma {
     static constexpr int kSpare = kAtOnce > 1 ? kTile * 8 * 4 : 0;
     const int lane, own, part, column;       // own: the head whose sums the lane gets; part: which of the positions at once; first columns: column and D / 2 + column
     const uint32_t weights;                  // shared memory: [position][8] (where a warp has all of a position, from lane to lane)
-    float q[HEADS][8], acc[HEADS][8], x[kSteps], m, l;       // scores, then weights, m and l of head `own`
+    float2 q[HEADS][4], acc[HEADS][4];       // by twos: one instruction for two
+    float x[kSteps], m, l;       // scores, then weights, m and l of head `own`
 
     QD_DEVINL PagedFma(int lane, uint32_t spare) : lane(lane),
         own(HEADS == 8 ? (lane & 1) * 4 + (lane >> 1 & 1) * 2 + (lane >> 2 & 1) : (lane & 1) * 2 + (lane >> 1 & 1)),
@@ -27,10 +28,10 @@ template <int D, int HEADS> struct PagedFma {
         return v;
     }
     // Eight columns of a row of a tile.
-    QD_DEVINL void row8(uint32_t tile, int row, float (&v)[8]) const {
+    QD_DEVINL void row8(uint32_t tile, int row, float2 (&v)[4]) const {
         const uint32_t at = tile + row * (D * 4) + (((lane % kLanes) ^ (row & 7)) << 4);
         const float4 a = shared4(at), b = shared4(at + D * 2);               // (kLanes pieces further: a multiple of eight)
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w); v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
     }
     QD_DEVINL void begin(uint32_t queries) {
 #pragma unroll
@@ -38,7 +39,7 @@ template <int D, int HEADS> struct PagedFma {
 #pragma unroll
         for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[h][j] = 0.f;
+            for (int j = 0; j < 4; ++j) acc[h][j] = make_float2(0.f, 0.f);
         m = -INFINITY; l = 0.f;
     }
     static QD_DEVINL constexpr int lane_of(int h) { return HEADS == 8 ? (h >> 2) + (h & 2) + (h & 1) * 4 : (h >> 1) + (h & 1) * 2; }       // that gets head h
@@ -62,13 +63,15 @@ template <int D, int HEADS> struct PagedFma {
         float top = -INFINITY;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            float k[8], v[HEADS];
+            float2 k[4];
+            float v[HEADS];
             row8(keys, s * kAtOnce + part, k);
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
-                v[h] = q[h][0] * k[0];
+                float2 sum = mul2(q[h][0], k[0]);
 #pragma unroll
-                for (int j = 1; j < 8; ++j) v[h] += q[h][j] * k[j];
+                for (int j = 1; j < 4; ++j) sum = fma2(q[h][j], k[j], sum);
+                v[h] = sum.x + sum.y;
             }
             x[s] = sum_up(v);
         }
@@ -89,7 +92,7 @@ template <int D, int HEADS> struct PagedFma {
             for (int h = 0; h < HEADS; ++h) {
                 const float of = __shfl_sync(0xffffffffu, fix, lane_of(h));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[h][j] *= of;
+                for (int j = 0; j < 4; ++j) acc[h][j] = mul2(acc[h][j], make_float2(of, of));
             }
         }
 #pragma unroll
@@ -105,7 +108,8 @@ template <int D, int HEADS> struct PagedFma {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int row = s * kAtOnce + part;
-            float v[8], w[8];
+            float2 v[4];
+            float w[8];
             row8(values, row, v);
             if constexpr (kAtOnce > 1) {
                 const float4 a = shared4(weights + row * 32), b = HEADS == 8 ? shared4(weights + row * 32 + 16) : a;
@@ -117,7 +121,7 @@ template <int D, int HEADS> struct PagedFma {
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[h][j] += w[h] * v[j];
+                for (int j = 0; j < 4; ++j) acc[h][j] = fma2(make_float2(w[h], w[h]), v[j], acc[h][j]);
         }
     }
     QD_DEVINL void leave(int, float* state, float2* stats) {
@@ -127,15 +131,18 @@ template <int D, int HEADS> struct PagedFma {
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[h][j] += __shfl_xor_sync(0xffffffffu, acc[h][j], e);
+                for (int j = 0; j < 4; ++j) {
+                    acc[h][j].x += __shfl_xor_sync(0xffffffffu, acc[h][j].x, e);
+                    acc[h][j].y += __shfl_xor_sync(0xffffffffu, acc[h][j].y, e);
+                }
         }
         if (lane < HEADS) stats[own] = make_float2(m, l);
         if (part == 0) {
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
                 float* to = state + h * D + (column ^ ((h >> 1) << 3));
-                *reinterpret_cast<float4*>(to) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
-                *reinterpret_cast<float4*>(to + D / 2) = make_float4(acc[h][4], acc[h][5], acc[h][6], acc[h][7]);
+                *reinterpret_cast<float4*>(to) = make_float4(acc[h][0].x, acc[h][0].y, acc[h][1].x, acc[h][1].y);
+                *reinterpret_cast<float4*>(to + D / 2) = make_float4(acc[h][2].x, acc[h][2].y, acc[h][3].x, acc[h][3].y);
             }
         }
     }
