@@ -6,12 +6,12 @@ namespace qd {
 
 // HEADS (4 or 8) query heads.  What bounds it is the number of instructions, 2 * HEADS * 4 of them multiply-adds for two rows' eight columns; so a sum
 // over lanes is taken for all heads at once, each step halving the heads that a lane still carries, and weights go through shared memory.  48 sequences
-// that see 1028 rows, 16 heads on 4 of 64 (99 MB): 23 us; 20 up to 3000, 32 on 8 of 128 (249 MB): 60; 16 up to 8000, 32 on 1 of 256 (138 MB, four
+// that see 1028 rows, 16 heads on 4 of 64 (99 MB, from HBM): 28 us; 20 up to 3000, 32 on 8 of 128 (249 MB): 60; 16 up to 8000, 32 on 1 of 256 (138 MB, four
 // passes over eight heads): 111, where arithmetic is all (134 with one multiply-add an instruction).
 template <int D, int HEADS> struct PagedFma {
     using Type = float;
     static constexpr int kDim = D, kHeads = 8, kTile = 8, kSeqs = 256;
-    static constexpr bool kNarrow = D == 64 && HEADS == 4;               // state and queries fit 128 registers: 23.2 us of the first, 28.4 by eight warps; eight heads of 64 would not, 79 for 35
+    static constexpr bool kNarrow = D == 64 && HEADS == 4;               // state and queries fit 128 registers: 28.2 us of the first, 29.4 by eight warps, 8 on 8 of 64 (370 MB) 73 and 80; eight heads of 64 would not, 79 for 35
     static constexpr int kWarps = kNarrow ? 16 : 8, kAhead = D == 256 ? 1 : D == 128 || kNarrow ? 2 : 4;
     static constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kSteps = kTile / kAtOnce;        // lanes of a position, positions at once
     static constexpr int kSpare = kAtOnce > 1 ? kTile * 8 * 4 : 0;

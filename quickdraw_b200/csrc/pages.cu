@@ -277,7 +277,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) rese
 }
 
 // The moves' rows, of every layer of both pools: a warp per 2 KB, four pieces of a lane in flight.  Bound by HBM: 1.38 GB in 215 us (6.4 TB/s), 72 MB
-// in pieces of one page 12 us.
+// in pieces of one page 16 us.
 struct MoveParams {
     char* k; char* v; const int* scratch; const int* list;
     long long page_bytes, layer_bytes, row_bytes;
