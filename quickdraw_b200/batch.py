@@ -179,13 +179,15 @@ class BatchDecode(ChunkPrefill):
         also loads and configures every kernel), the second captures, later ones replay; the
         results live in buffers that the next call overwrites.  ``state.positions`` may only be
         written by the steps themselves once a state has been captured (call ``forget`` after
-        writing them)."""
+        writing them).  After a resize of its pages a state begins anew: a call that runs eagerly, one
+        that captures."""
         entry = self._graphs.get(id(state))
-        if entry is None:
+        pools = state.cache.resized if isinstance(state, PagedBatchState) else 0
+        if entry is None or entry["pools"] != pools:
             out = self.step(tokens, state)
             # host-side bound of the largest position: the device value is read again only when
             # the bound reaches the end of the cache
-            self._graphs[id(state)] = {"state": state, "bound": int(state.positions.max().item()), "graph": None}
+            self._graphs[id(state)] = {"state": state, "bound": int(state.positions.max().item()), "graph": None, "pools": pools}
             return out
         if entry["bound"] >= state.max_context:
             entry["bound"] = int(state.positions.max().item())

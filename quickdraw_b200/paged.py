@@ -190,7 +190,7 @@ class PagedCache:
     """Pools of ``pages`` pages for ``layers`` attention layers, tables of ``sequences`` sequences of at most ``max_context`` rows.
 
     ``k``, ``v`` [pages, layers, page, kv_heads, head_dim]; ``table``, ``lengths``, ``refs``, ``status`` int32 on the device.  The methods
-    write into these tensors, which a captured graph may therefore hold; ``resize`` alone replaces the pools."""
+    write into these tensors, which a captured graph may therefore hold; ``resize`` alone replaces ``k``, ``v`` and ``refs``."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int, sequences: int, max_context: int, device,
                  dtype: torch.dtype = BF16):
@@ -202,6 +202,7 @@ class PagedCache:
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.resized = 0                    # how often: a graph that was captured before the last time must not run any more
 
     @property
     def pages(self) -> int:
@@ -233,7 +234,8 @@ class PagedCache:
 
     def resize(self, pages: int) -> None:
         """Pools of ``pages`` pages, at least as many as are in use: what is not used is given back, or there is more of it.  Waits for
-        the device; graphs captured with the old pools go on using those."""
+        the device.  A graph captured before has the addresses of the old pools, whose memory is given back, and must not be replayed:
+        ``BatchDecode.graph_step`` sees to its own; ``resized`` counts."""
         assert pages > 0
         used = int(self.compact().item())
         assert pages >= used, f"{used} pages are in use"
@@ -243,6 +245,7 @@ class PagedCache:
             new = torch.zeros((pages, *old.shape[1:]), dtype=old.dtype, device=old.device)
             new[:kept] = old[:kept]
             setattr(self, name, new)
+        self.resized += 1
 
     def _rows(self, b: int, k: torch.Tensor, v: torch.Tensor, first: int, count: int, out: bool) -> None:
         pages, layers, page, heads, dim = self.k.shape

@@ -460,3 +460,27 @@ def test_a_pool_that_is_too_small_is_said(cuda_device):
     state = paged.PagedBatchState(cfg, 2, 64, "cuda", pages=1, page=16)
     with pytest.raises(AssertionError, match="no free page"):
         decoder.step(torch.tensor([3, 5], device="cuda"), state)
+
+
+def test_a_captured_step_goes_on_after_a_resize(cuda_device):
+    """Pools that get smaller, and larger, between replayed steps; what the old ones' memory holds now stays as it is."""
+    from quickdraw_b200.batch import BatchDecode
+    cfg, ckpt = small_model()
+    decoder = BatchDecode(ckpt)
+    runs, others = [], []
+    for method in (decoder.step, decoder.graph_step):
+        state = paged.PagedBatchState(cfg, 3, 60, "cuda", pages=24, page=8)
+        tokens, seen = torch.tensor([3, 5, 8], device="cuda"), []
+        for step in range(24):
+            picked, logits = method(tokens, state)
+            seen.append((picked.clone(), logits.clone()))
+            tokens = picked.clone()
+            if step in (7, 15):
+                was = state.cache.k.numel()
+                state.cache.resize(12 if step == 7 else 20)
+                others.append(torch.full((was,), 7.0, dtype=BF16, device="cuda"))
+        assert state.cache.check() == 0 and int(state.cache.refs.sum()) == int((state.cache.table >= 0).sum()) == 9
+        runs.append(seen)
+    for (a, x), (b, y) in zip(*runs):
+        assert torch.equal(a, b) and torch.equal(x, y)
+    assert all(bool((t == 7.0).all()) for t in others)

@@ -205,3 +205,29 @@ def test_plain_forms_agree_with_themselves():
     q = torch.randn(4, 2, 8, generator=torch.Generator().manual_seed(1))[:1].expand(4, 2, 8)
     out, bound = plain.attention(q, new[0][:, 0], new[1][:, 0], new[2], new[3])
     assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[3]) and not math.isnan(float(out.sum())) and float(bound.max()) < 1e-2
+
+
+def test_a_captured_step_is_not_replayed_after_a_resize(monkeypatch):
+    """Its kernels have the addresses of pools whose memory was given back."""
+    import contextlib
+    from types import SimpleNamespace
+
+    from quickdraw_b200 import batch
+    done = []
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: SimpleNamespace(replay=lambda: done.append("replay")))
+    monkeypatch.setattr(torch.cuda, "graph", lambda graph: contextlib.nullcontext())
+    monkeypatch.setattr(batch, "lib", lambda: SimpleNamespace(qd_set_chained_launches=lambda on: 1))
+    monkeypatch.setattr(paged, "compact_pages", lambda k, v, table, refs: (table.clone(), refs.clone(), torch.zeros((), dtype=I32)))
+    decoder = batch.BatchDecode.__new__(batch.BatchDecode)
+    decoder._graphs = {}
+    monkeypatch.setattr(decoder, "step", lambda tokens, state, positions_checked=False: done.append("capture" if positions_checked else "eager"), raising=False)
+    state, tokens = paged.PagedBatchState(synthetic.model_config(num_layers=4, vocab_size=64), 2, 64, "cpu", page=16), torch.zeros(2, dtype=torch.long)
+    for _ in range(3):
+        decoder.graph_step(tokens, state)
+    assert done == ["eager", "capture", "replay", "replay"]
+    for pages in (5, 5, 9):
+        done.clear()
+        state.cache.resize(pages)
+        for _ in range(3):
+            decoder.graph_step(tokens, state)
+        assert done == ["eager", "capture", "replay", "replay"], pages
