@@ -136,7 +136,8 @@ QD_DEVINL void fork_pages(const ForkParams& p) {
     int wanted = 0;
     for (int base = 0; base < S; base += kThreads) {
         const int b = base + tid, parent = b < S ? parent_of[b] : -1, n = b < S ? length(b) : 0;
-        const bool asking = parent >= 0 && parent != b && n % p.page != 0 && first[parent] != b;
+        // (a parent without that page, of which nothing is seen, has children without it: a free page would show them what its last owner left)
+        const bool asking = parent >= 0 && parent != b && n % p.page != 0 && first[parent] != b && is_page(p.table[(long long)parent * p.width + n / p.page], p.pages);
         if (b < S && blockIdx.x == 0) p.lengths_out[b] = n;
         int found;
         const int rank = wanted + block_before(asking, &found, sums);
@@ -148,10 +149,9 @@ QD_DEVINL void fork_pages(const ForkParams& p) {
     const Run run = list_count<BLOCKS>(p.pages, p.scratch + kCounts, sums, free_page);
     list_found(run, wanted, free_page, [&](int rank, int page) {
         const int b = asks[rank], parent = parent_of[b], n = length(b), full = n / p.page;
-        const int tail = p.table[(long long)parent * p.width + full];
         p.table_out[(long long)b * p.width + full] = page;
         p.refs_out[page] = 1;                                           // (looked at by this warp alone)
-        moves[rank] = Move{tail, page, is_page(tail, p.pages) ? n - full * p.page : 0};
+        moves[rank] = Move{p.table[(long long)parent * p.width + full], page, n - full * p.page};
     });
     if (blockIdx.x) return;
     const int got = min(wanted, run.total);

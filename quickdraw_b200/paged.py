@@ -141,7 +141,8 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     """Sequence b goes on as a copy of sequence ``parents[b]``, all at once: the new (table, lengths, refs).  -1: the sequence ends
     and gives up its pages; its own number: it stays as it is.  Full pages are shared.  A page that is not full goes to the parent
     itself where that stays, or else to the lowest child; every other child gets the lowest free page and a copy of its rows, in
-    the order of the children.  Only those rows are written, in ``k_pages`` and ``v_pages`` [pages, layers, page, kv_heads, dim].
+    the order of the children.  Only those rows are written, in ``k_pages`` and ``v_pages`` [pages, layers, page, kv_heads, dim].  Rows that
+    the parent has no page for (they are not seen) no child has a page for either.
 
     A parent that is no sequence leaves its child as it is, and a child for which no page is left ends where its full pages do; both
     set bits of ``status`` (int32 [1]; a word shared by the device, ``device_status``, if not given)."""

@@ -257,6 +257,30 @@ def test_fork_without_room_and_with_parents_that_are_none(cuda_device):
             assert torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7)), parents
 
 
+@pytest.mark.parametrize("hole", [-1, -9, 2 ** 31 - 1])
+@pytest.mark.parametrize("parents", [[0, 0, 0, 3], [1, 0, 0, 0], [3, 3, 0, -1], [0, 1, 2, 3]])
+def test_fork_of_a_sequence_without_its_last_page(cuda_device, parents, hole):
+    """Rows that the parent does not see, its copies do not see either: no page with what its last owner left there (NaN here)."""
+    page, lengths = 16, [37, 20, 16, 50]
+    k, v, table, n, refs = plain.cache(lengths, page, 1, 1, 64, BF16, seed=3, spare=10)
+    refs[table[0, 2].long()] -= 1
+    table[0, 2] = hole
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = [t.clone() for t in (k, v, table, n)]
+    new = paged.fork_pages(k, v, table, n, refs, torch.tensor(parents, dtype=torch.int32, device="cuda"), status=status)
+    assert int(status) == 0 and new[1].tolist() == [lengths[p] if p >= 0 else 0 for p in parents]
+    held = new[0][(new[0] >= 0) & (new[0] < refs.numel())].long()
+    assert torch.equal(torch.bincount(held, minlength=refs.numel()).int(), new[2])
+    for b, p in enumerate(parents):
+        if p == 0:
+            assert torch.equal(new[0][b, :2], table[0, :2]) and not 0 <= int(new[0][b, 2]) < refs.numel()
+    q = torch.randn((1, 2, 64), generator=torch.Generator().manual_seed(3)).to(BF16).cuda().expand(4, 2, 64)
+    was = paged.paged_attention(q, before[0][:, 0], before[1][:, 0], *before[2:])
+    now = paged.paged_attention(q, k[:, 0], v[:, 0], *new[:2])
+    for b, p in enumerate(parents):
+        assert torch.equal(now[b], was[p] if p >= 0 else torch.zeros_like(now[b])), (b, p)
+
+
 @pytest.mark.parametrize("lengths,spare", [([5, 700, 0, 64], 60), ([16], 0), ([1], 5000), ([0, 0], 7), ([100] * 40, 130)])
 def test_compact(cuda_device, lengths, spare):
     for page, layers, heads, dim, dtype in ((16, 2, 2, 64, BF16), (1, 1, 1, 8, F32), (24, 1, 5, 40, BF16)):
