@@ -280,9 +280,11 @@ int qd_pages_compact(void* k, void* v, long long page_bytes, long long layer_byt
                      const int* table, const int* refs, int* table_out, int* refs_out, int* used, int* scratch,
                      int sequences, int width, int pages, int page, void* stream);
 
-/* Pages for the next counts[b] rows of every sequence (counts NULL: `count`), in place, the lowest free ones in order. */
+/* Pages for the next counts[b] rows of every sequence (counts NULL: `count`), in place, the lowest free ones in order.  The page
+ * of a row that has others of its sequence in front of it was given before: it is never given anew, and where it is missing
+ * begun = 1 sets the bit of a missing page in status. */
 int qd_pages_reserve(int* table, const int* lengths, int* refs, const int* counts, int count, int* scratch,
-                     unsigned int* status, int sequences, int width, int pages, int page, void* stream);
+                     unsigned int* status, int sequences, int width, int pages, int page, int begun, void* stream);
 
 /* Rows first .. first + count - 1 of one sequence (table: its row) of every layer from k_rows, v_rows (contiguous rows of
  * layers rows_layer_bytes apart) to the pool, or (out = 1) from the pool to them. */

@@ -84,7 +84,7 @@ SIGNATURES = {
     "qd_pages_scratch_words": [I, I, I],
     "qd_pages_fork": [P, P, L, L, L, I, P, P, P, P, P, P, P, P, P, I, I, I, I, P],
     "qd_pages_compact": [P, P, L, L, L, I, P, P, P, P, P, P, I, I, I, I, P],
-    "qd_pages_reserve": [P, P, P, P, I, P, P, I, I, I, I, P],
+    "qd_pages_reserve": [P, P, P, P, I, P, P, I, I, I, I, I, P],
     "qd_pages_rows": [P, P, L, L, L, P, P, L, P, P, I, I, I, I, I, I, I, P],
     "qd_beam_scratch_bytes": [I, I, I, I],
     "qd_beam_select": [P, L, I, P, P, I, P, P, P, P, I, I, I, I, I, P],

@@ -228,7 +228,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) comp
 
 struct ReserveParams {
     int* table; const int* lengths; int* refs; const int* counts; int* scratch; unsigned int* status;
-    int count, sequences, width, pages, page;
+    int count, sequences, width, pages, page, begun;
 };
 // One block, or (many pages) a cluster whose blocks all list the requests.
 template <int BLOCKS>
@@ -247,6 +247,9 @@ QD_DEVINL void reserve_pages(const ReserveParams& p) {
             } else if (more > 0) {
                 from = n ? (n - 1) / p.page + 1 : 0;
                 to = (n + more - 1) / p.page + 1;                           // (no sum passes the table's rows)
+                // a page in whose middle the sequence is cannot be made up for (what was to be in front is lost), nor are the rows to come there
+                if (p.begun && blockIdx.x == 0 && n % p.page && !is_page(read_now(p.table + (long long)b * p.width + n / p.page), p.pages))
+                    atomicOr(p.status, QD_STATUS_NO_PAGE);
                 for (int j = from; j < to; ++j) need += read_now(p.table + (long long)b * p.width + j) < 0;
             }
         }
@@ -388,10 +391,10 @@ extern "C" int qd_pages_compact(void* k, void* v, long long page_bytes, long lon
 }
 
 extern "C" int qd_pages_reserve(int* table, const int* lengths, int* refs, const int* counts, int count, int* scratch, unsigned int* status,
-                                int sequences, int width, int pages, int page, void* stream) {
+                                int sequences, int width, int pages, int page, int begun, void* stream) {
     QD_CHECK_ARG(table && lengths && refs && scratch && status && (counts || count >= 0));
     QD_CHECK_ARG(sequences > 0 && width > 0 && pages > 0 && page > 0 && (long long)sequences * width <= 0x7fffffffll);
-    ReserveParams p{table, lengths, refs, counts, scratch, status, count, sequences, width, pages, page};
+    ReserveParams p{table, lengths, refs, counts, scratch, status, count, sequences, width, pages, page, begun};
     return few(sequences, pages) ? qd_launch(reserve_block_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, 3, p)
                                  : qd_launch(reserve_cluster_kernel, dim3(kBlocks), dim3(kThreads), 0, (cudaStream_t)stream, 3, p);
 }

@@ -172,9 +172,13 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     return table_out, refs_out, used
 
 
-def reserve_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, page: int, counts=1, *, status: torch.Tensor | None = None) -> None:
+def reserve_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, page: int, counts=1, *, begun: bool = False,
+                  status: torch.Tensor | None = None) -> None:
     """Pages for the next ``counts`` rows (a number, or int32 [sequences] on the device) of every sequence, in place in ``table`` and
-    ``refs``: the lowest free ones, in the order of the sequences.  Rows past the table and an empty pool set bits of ``status``."""
+    ``refs``: the lowest free ones, in the order of the sequences.  Rows past the table and an empty pool set bits of ``status``.
+
+    A page is given for its first row: where the pool had none then, the sequence has none for the page's other rows, which are lost like
+    the first.  ``begun``: that sets the bit of an empty pool too, as long as such rows are asked for."""
     assert table.is_cuda
     device = table.get_device()
     count, width, pages, scratch = _check_tables(table, refs, device)
@@ -184,7 +188,7 @@ def reserve_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor
     status = device_status(table.device) if status is None else status
     assert _is_ids(status, device, 1)
     launch(table, "qd_pages_reserve", ptr(table), ptr(lengths), ptr(refs), ptr(counts) if each else None, 0 if each else int(counts),
-           ptr(scratch), ptr(status), count, width, pages, page)
+           ptr(scratch), ptr(status), count, width, pages, page, int(begun))
 
 
 class PagedCache:
@@ -210,8 +214,9 @@ class PagedCache:
         return self.refs.numel()
 
     def reserve(self, counts=1) -> None:
-        """Room for the next ``counts`` rows of every sequence (``reserve_pages``)."""
-        reserve_pages(self.table, self.lengths, self.refs, self.page, counts, status=self.status)
+        """Room for the next ``counts`` rows of every sequence (``reserve_pages``); each call that leaves some without a page says so in
+        ``status``."""
+        reserve_pages(self.table, self.lengths, self.refs, self.page, counts, begun=True, status=self.status)
 
     def fork(self, parents: torch.Tensor) -> None:
         """Sequence b goes on as a copy of sequence ``parents[b]`` (``fork_pages``)."""

@@ -318,6 +318,39 @@ def test_reserve_of_pages_as_long_as_numbers_go(cuda_device):
     assert table.tolist() == [[0], [-1]] and int(status) == paged.BAD_ARGUMENT
 
 
+@pytest.mark.parametrize("sequences", [2, 1100, 9000])
+def test_every_row_without_a_page_is_said(cuda_device, sequences):
+    """A pool that was empty at a page's first row: each of the page's other rows is lost too, and each time the status says so."""
+    page = 4
+    cache = paged.PagedCache(1, 1, 8, sequences - 1, page, sequences, 16, "cuda")
+    words = []
+    for step in range(3 * page):
+        if step == page + 1:
+            cache.free([0])                                            # its place takes the page again; the last one is in the middle of one
+        cache.reserve()
+        words.append(cache.check())
+        cache.lengths += 1
+    assert words[:page] == [paged.NO_PAGE] * page and cache.table[-1, 0] == -1
+    assert words[page] == paged.NO_PAGE and words[page + 1:2 * page] == [paged.NO_PAGE] * (page - 1)
+    last = cache.lengths[-1:].clone()
+    # nothing is said of a sequence that asks for no row, of a full page, and by the tables' own form without `begun`
+    only = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+    cache.lengths.fill_(page), cache.table.fill_(-1), cache.refs.zero_()
+    cache.reserve(only)
+    assert cache.check() == 0
+    only[0] = 1
+    cache.reserve(only)
+    assert cache.check() == 0 and cache.table[0].tolist() == [-1, 0, -1, -1] and int(last) == 3 * page
+    cache.lengths.fill_(page + 1)
+    paged.reserve_pages(cache.table, cache.lengths, cache.refs, page, only, status=cache.status)
+    assert cache.check() == 0
+    cache.reserve(only)
+    assert cache.check() == 0
+    only[1] = 1
+    cache.reserve(only)
+    assert cache.check() == paged.NO_PAGE and cache.table[1].tolist() == [-1] * 4
+
+
 def test_forks_and_reservations_from_a_graph(cuda_device):
     def life(cache, state, parents, fork):
         fork()
@@ -484,6 +517,21 @@ def test_a_pool_that_is_too_small_is_said(cuda_device):
     state = paged.PagedBatchState(cfg, 2, 64, "cuda", pages=1, page=16)
     with pytest.raises(AssertionError, match="no free page"):
         decoder.step(torch.tensor([3, 5], device="cuda"), state)
+
+
+def test_a_captured_step_says_each_row_that_is_lost(cuda_device):
+    from quickdraw_b200.batch import BatchDecode
+    cfg, ckpt = small_model()
+    decoder = BatchDecode(ckpt)
+    state, words = paged.PagedBatchState(cfg, 2, 32, "cuda", pages=3, page=4), []
+    tokens = torch.tensor([3, 5], device="cuda")
+    for step in range(14):
+        if step == 10:
+            state.free([0])                                     # two pages: for its place's row 0 and for the second's row 12
+        decoder.graph_step(tokens, state)
+        words.append(state.cache.check())
+    # rows 4 to 11 of the second have no page
+    assert words == [0] * 4 + [paged.NO_PAGE] * 8 + [0] * 2
 
 
 def test_a_captured_step_goes_on_after_a_resize(cuda_device):
