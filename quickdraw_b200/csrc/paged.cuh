@@ -98,7 +98,7 @@ struct PagedParams {
     long long q_row, q_head, gate_row, gate_head, page_stride, row_stride, head_stride, table_stride;   // in elements
     const int* table; const int* lengths;
     void* out;                          // [batch, heads, dim]
-    float* partial; float2* stats;      // [pair][most][heads of a chunk][dim]: weighted values; [pair][most][heads of a chunk]: maximum, sum
+    float* partial; float2* stats;      // [pair][most][heads of a chunk][dim]: weighted means; [pair][most][heads of a chunk]: maximum, sum
     int batch, heads, kv_heads, dim, pages, page, width, window, sinks;
     int group, chunk, chunks;           // query heads of a key/value head; of them at a time; how often
     int unit;                           // positions of a unit

@@ -7,7 +7,7 @@
 namespace qd {
 namespace {
 
-// The parts of a (sequence, head) joined, 32 * EACH columns by WARPS warps that take every WARPS-th part; a sequence that sees nothing gets zeros.
+// The means of a (sequence, head)'s parts joined, 32 * EACH columns by WARPS warps that take every WARPS-th part; a sequence that sees nothing gets zeros.
 constexpr int kJoinWarps = 8;
 template <typename T, int EACH, int WARPS>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p) {
@@ -23,48 +23,52 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
     int mine = warp + lane * WARPS;                                    // a lane's part
     float2 of = mine < p.cuts.most ? p.stats[place + (long long)mine * p.chunk] : make_float2(0.f, 0.f);
     const int parts = paged_parts(p.cuts, paged_span(p, b).seen, p.unit);
-    float top = -INFINITY, den = 0.f, num[EACH] = {};
+    float top = -INFINITY, den = 0.f, mean[EACH] = {};
     for (int base = warp; base < parts; base += 32 * WARPS) {
         if (base != warp) of = mine < parts ? p.stats[place + (long long)mine * p.chunk] : of;
         if (mine >= parts) of = make_float2(-INFINITY, 0.f);
         const float now = fmaxf(top, warp_max(of.x)), shift = now == -INFINITY ? 0.f : now;
-        const float fix = exp2f(top - shift), w = of.y == 0.f ? 0.f : exp2f(of.x - shift);
+        const float w = of.y == 0.f ? 0.f : exp2f(of.x - shift) * of.y, before = den * exp2f(top - shift);
         top = now;
-        den = den * fix + warp_sum(w * of.y);
+        den = before + warp_sum(w);
+        const float inverse = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) num[j] *= fix;
+        for (int j = 0; j < EACH; ++j) mean[j] *= before * inverse;
         const int count = min(32, (parts - base + WARPS - 1) / WARPS);
 #pragma unroll (EACH > 2 ? 2 : 16)
         for (int i = 0; i < count; ++i) {
-            const float each_w = __shfl_sync(0xffffffffu, w, i);
+            const float share = __shfl_sync(0xffffffffu, w * inverse, i);
             const float* from = src + (long long)(base + i * WARPS) * p.chunk * p.dim;
 #pragma unroll
             for (int j = 0; j < EACH; ++j)
-                if (column + j * 32 < p.dim) num[j] += each_w * from[j * 32];
+                if (column + j * 32 < p.dim) mean[j] += share * from[j * 32];
         }
         mine += 32 * WARPS;
     }
     if constexpr (WARPS == 1) {
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
-            if (column + j * 32 < p.dim) paged_put<T>(p, b, head, column + j * 32, den == 0.f ? 0.f : num[j] / den);
+            if (column + j * 32 < p.dim) paged_put<T>(p, b, head, column + j * 32, mean[j]);
     } else {
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) state[warp][j * 32 + lane] = num[j];
+    for (int j = 0; j < EACH; ++j) state[warp][j * 32 + lane] = mean[j];
     if (lane == 0) { state[warp][EACH * 32] = top; state[warp][EACH * 32 + 1] = den; }
     __syncthreads();
     const int f = blockIdx.y * EACH * 32 + tid;
     if (tid >= EACH * 32 || f >= p.dim) return;
-    float all = -INFINITY, sum = 0.f, v = 0.f;
+    float all = -INFINITY, sum = 0.f, v = 0.f, share[WARPS];
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) all = fmaxf(all, state[w][EACH * 32]);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        const float g = state[w][EACH * 32 + 1] == 0.f ? 0.f : exp2f(state[w][EACH * 32] - all);
-        sum += g * state[w][EACH * 32 + 1];
-        v += g * state[w][tid];
+        const float of_w = state[w][EACH * 32 + 1];
+        share[w] = of_w == 0.f ? 0.f : exp2f(state[w][EACH * 32] - all) * of_w;
+        sum += share[w];
     }
-    paged_put<T>(p, b, head, f, sum == 0.f ? 0.f : v / sum);
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v += share[w] * inverse * state[w][tid];
+    paged_put<T>(p, b, head, f, v);
     }
 }
 

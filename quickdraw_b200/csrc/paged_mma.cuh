@@ -110,7 +110,8 @@ template <int D, int NT> struct PagedMma {
             for (int e = 0; e < 4; ++e) x[e] = weight_of(x[e], m[n][e & 1]);
             l[n][0] += x[0] + x[2];
             l[n][1] += x[1] + x[3];
-            // weights in two bf16 pieces (sixteen bits): one alone would be off by as much as the result's own rounding
+            // weights in two bf16 pieces (sixteen bits): one alone would be off by as much as the result's own rounding (of an infinite
+            // value they may make NaN: such sums are formed again)
             const uint32_t h0 = pack2(x[0], x[1]), h1 = pack2(x[2], x[3]);
             hi[n][0] = transposed(h0); hi[n][1] = transposed(h1);
             lo[n][0] = transposed(pack2(x[0] - low_of(h0), x[1] - high_of(h0)));
@@ -129,6 +130,16 @@ template <int D, int NT> struct PagedMma {
             }
         });
     }
+    QD_DEVINL bool unbounded() const {
+        float odd = 0.f;                                               // zero times what is not finite is NaN
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd = fmaf(acc[n][d][e], 0.f, odd);
+        return odd != 0.f;
+    }
     QD_DEVINL void leave(int n, float* state, float2* stats) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -136,10 +147,11 @@ template <int D, int NT> struct PagedMma {
             for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
             const int h = 2 * t + e;
             if (g == 0) stats[h] = make_float2(m[n][e], l[n][e]);
+            const float inverse = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-                for (int up = 0; up < 2; ++up) state[h * D + ((d * 16 + up * 8 + g) ^ (t << 3))] = acc[n][d][2 * up + e];
+                for (int up = 0; up < 2; ++up) state[h * D + ((d * 16 + up * 8 + g) ^ (t << 3))] = acc[n][d][2 * up + e] * inverse;
         }
     }
 };

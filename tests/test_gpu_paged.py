@@ -91,6 +91,49 @@ def test_scores_far_apart_and_infinite(cuda_device, dtype):
     assert bool(torch.isnan(out[2, :2]).all()) and bool(torch.isfinite(out[2, 2:]).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+def test_infinite_and_largest_values(cuda_device, heads, kv_heads, dim, dtype):
+    """An infinity among the values is the mean of its column, those of both signs and NaN give NaN there, and means of the largest numbers stay below
+    them; the other columns do not notice.  One launch and two, one row and many, pages that are missing between them."""
+    largest = 3.3e38
+    for lengths, page, width in (([1, 2, 40, 0], 16, 4), ([700, 1, 333, 64], 16, None)):
+        q, k, v, table, n, _ = problem(lengths, heads, kv_heads, dim, page, dtype, seed=dim, width=width)
+        inside, last = table.cpu(), [n - 1 for n in lengths]
+        at = lambda b, p: (int(inside[b, p // page]), p % page)  # noqa: E731
+        clean = v.clone()
+        for t in (v, clean):
+            for b in (0, 2):
+                for p in range(lengths[b]):
+                    t[at(b, p)][:, 1] = largest if p % 7 else largest / 2           # a column of them
+                    t[at(b, p)][:, 4] = largest if p % 2 else -largest
+        for b in (0, 2):
+            v[at(b, last[b])][:, 2], clean[at(b, last[b])][:, 2] = math.inf, 0.0
+            v[at(b, 0)][:, 3], clean[at(b, 0)][:, 3] = -math.inf, 0.0
+            v[at(b, last[b])][:, 5], clean[at(b, last[b])][:, 5] = math.nan, 0.0
+            v[at(b, last[b] // 2)][0, 6], clean[at(b, last[b] // 2)][0, 6] = math.inf, 0.0
+            v[at(b, last[b])][:, 7], clean[at(b, last[b])][:, 7] = math.inf, 0.0
+            if last[b]:
+                v[at(b, 0)][:, 7], clean[at(b, 0)][:, 7] = -math.inf, 0.0
+        for seen in (dict(), dict(window=30, sinks=2)):
+            got = paged.paged_attention(q, k, v, table, n, **seen)
+            want, bound = plain.attention(q, k, clean, table, n, **seen)
+            for b in (0, 2):
+                want[b, :, 2], want[b, :, 3], want[b, :, 5] = math.inf, -math.inf, math.nan
+                if not seen or last[b] // 2 < 2 or last[b] - last[b] // 2 < 30:
+                    want[b, :heads // kv_heads, 6] = math.inf
+                want[b, :, 7] = math.nan if last[b] else math.inf
+            got, fine = got.cpu().double(), torch.isfinite(want)
+            assert torch.equal(torch.nan_to_num(got[~fine], nan=5.0), torch.nan_to_num(want[~fine], nan=5.0)), (lengths, seen)
+            assert bool(torch.isfinite(got[fine]).all()) and bool(((got - want).abs() <= bound)[fine].all()), (lengths, seen)
+            # the bound of a column of such values says nothing of the others
+            small = clean.clone()
+            small[..., 1], small[..., 4] = 0.0, 0.0
+            want, bound = plain.attention(q, k, small, table, n, **seen)
+            columns = [0, *range(8, dim)]
+            assert bool(((got - want).abs() <= bound)[:, :, columns].all()), (lengths, seen)
+
+
 def test_views_with_other_strides(cuda_device):
     """Layers of one pool, pools with the heads outside of the rows, queries and gates inside a projection, a table inside a larger one."""
     lengths, page = [120, 77, 300], 16
