@@ -305,7 +305,7 @@ int qd_beam_select(const void* logits, long long row_stride, int is_fp32, const 
                    int candidates, int placed, void* stream);
 
 /* state[b] = old state[parents[b]] (-1: zeros; itself: not touched) of up to four tensors (NULL: none) of `sequences` rows of
- * row bytes, stride bytes apart. */
+ * row bytes, stride bytes apart.  At most 7000 sequences, else QD_ERR_UNSUPPORTED. */
 int qd_reorder_states(void* state0, long long row0, long long stride0, void* state1, long long row1, long long stride1,
                       void* state2, long long row2, long long stride2, void* state3, long long row3, long long stride3,
                       const int* parents, unsigned int* status, int sequences, void* stream);

@@ -12,6 +12,7 @@ from .state import DecodeState
 
 BF16 = torch.bfloat16
 MOST_BEAMS = 32
+MOST_ROWS = 7000            # that reorder_states puts in order at once
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.Tensor | None = None, eos: int | None = None,
@@ -48,10 +49,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
 
 def reorder_states(states, parents: torch.Tensor, *, status: torch.Tensor | None = None) -> None:
     """``state[b] = old state[parents[b]]`` in place, for tensors [sequences, ...] that do not overlap (rows contiguous, any distance apart): -1 is
-    a row of zeros, a row that is its own parent is not touched, one whose parent is no row neither (a bit of ``status``)."""
+    a row of zeros, a row that is its own parent is not touched, one whose parent is no row neither (a bit of ``status``).  At most 7000 rows."""
     states = [states] if isinstance(states, torch.Tensor) else list(states)
     assert parents.is_cuda and parents.ndim == 1 and _is_ids(parents, parents.get_device(), *parents.shape) and parents.numel() > 0
     device, count = parents.get_device(), parents.numel()
+    assert count <= MOST_ROWS, "1 to 7000 rows"
     status = device_status(parents.device) if status is None else status
     assert _is_ids(status, device, 1)
     rows = []

@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderP
 template <typename U>
 int reorder_launch(const ReorderParams& p, dim3 grid, size_t smem, cudaStream_t stream) {
     static bool raised[kDevices];
-    if (smem > 48 * 1024 && !raise_smem(reorder_kernel<U>, 200 * 1024, raised)) return QD_ERR_LAUNCH;
+    if (smem > 40 * 1024 && !raise_smem(reorder_kernel<U>, 200 * 1024, raised)) return QD_ERR_LAUNCH;        // (what is declared counts too)
     return qd_launch(reorder_kernel<U>, grid, dim3(kReorderThreads), smem, stream, 3, p);
 }
 

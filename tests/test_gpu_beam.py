@@ -161,6 +161,19 @@ def test_reorder_of_many_rows_apart(cuda_device):
         assert torch.equal(wide, want)
 
 
+@pytest.mark.parametrize("count", [1753, 1754, 1755, 1756, 7000])
+@pytest.mark.parametrize("dtype,row", [(F32, 4), (F32, 3), (BF16, 3), (torch.uint8, 5)])
+def test_reorder_of_as_many_rows_as_shared_memory_takes(cuda_device, count, dtype, row):
+    """Around the size from which a launch has to ask for more than it gets without asking, with units of 16, 4, 2 and 1 bytes; and the most."""
+    g = torch.Generator().manual_seed(1)
+    state = torch.randint(0, 100, (count, row), generator=g).to(dtype)
+    parents = torch.randint(-1, count, (count,), generator=g).int()
+    want = torch.where((parents >= 0)[:, None], state[parents.clamp(min=0).long()], 0)
+    got = state.cuda()
+    beam.reorder_states(got, parents.cuda())
+    assert torch.equal(got.cpu(), want.to(dtype))
+
+
 def test_reorder_with_parents_that_are_none(cuda_device):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     state = torch.arange(12.0, device="cuda").view(3, 4).clone()

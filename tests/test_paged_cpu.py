@@ -231,3 +231,12 @@ def test_a_captured_step_is_not_replayed_after_a_resize(monkeypatch):
         for _ in range(3):
             decoder.graph_step(tokens, state)
         assert done == ["eager", "capture", "replay", "replay"], pages
+
+
+def test_reorder_refuses_more_rows_than_it_holds(calls):
+    status = on_gpu(torch.zeros(1, dtype=I32))
+    beam.reorder_states(on_gpu(torch.zeros(7000, 1)), on_gpu(torch.zeros(7000, dtype=I32)), status=status)
+    assert calls.pop()[1][14] == 7000
+    with pytest.raises(AssertionError, match="7000"):
+        beam.reorder_states(on_gpu(torch.zeros(7001, 1)), on_gpu(torch.zeros(7001, dtype=I32)), status=status)
+    assert not calls
