@@ -269,7 +269,8 @@ long long qd_pages_scratch_words(int sequences, int width, int pages);
  * shared.  A page that is not full goes to the parent itself or else to its first child; the others, in order, get the lowest
  * free pages and a copy of its rows (nothing where the parent's entry is no page).  Pools: layers of [page, row], layer_bytes
  * and page_bytes apart, pieces of 16 bytes.  Pages that nobody uses any more keep what they hold.  The outputs are other arrays
- * than the inputs.  Without a free page a sequence ends where its full pages do (status). */
+ * than the inputs.  Without a free page a sequence ends where its full pages do (status).  At most 12800 sequences, else
+ * QD_ERR_UNSUPPORTED. */
 int qd_pages_fork(void* k, void* v, long long page_bytes, long long layer_bytes, long long row_bytes, int layers,
                   const int* table, const int* lengths, const int* refs, const int* parents, int* table_out,
                   int* lengths_out, int* refs_out, int* scratch, unsigned int* status, int sequences, int width, int pages,

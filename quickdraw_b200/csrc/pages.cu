@@ -368,8 +368,8 @@ extern "C" int qd_pages_fork(void* k, void* v, long long page_bytes, long long l
     if (smem > 200 * 1024) return QD_ERR_UNSUPPORTED;
     const bool alone = few((long long)sequences * width, pages);
     static bool raised_block[kDevices], raised_cluster[kDevices];
-    if (smem > 48 * 1024 && !(alone ? raise_smem(fork_block_kernel, 200 * 1024, raised_block) : raise_smem(fork_cluster_kernel, 200 * 1024, raised_cluster)))
-        return QD_ERR_LAUNCH;
+    if (smem > 40 * 1024 && !(alone ? raise_smem(fork_block_kernel, 200 * 1024, raised_block) : raise_smem(fork_cluster_kernel, 200 * 1024, raised_cluster)))
+        return QD_ERR_LAUNCH;                                              // (what is declared counts too)
     const int code = alone ? qd_launch(fork_block_kernel, dim3(1), dim3(kThreads), smem, (cudaStream_t)stream, 3, p)
                            : qd_launch(fork_cluster_kernel, dim3(kBlocks), dim3(kThreads), smem, (cudaStream_t)stream, 3, p);
     if (code != QD_OK) return code;

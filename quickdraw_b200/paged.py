@@ -27,6 +27,7 @@ from .state import DecodeState
 
 BF16 = torch.bfloat16
 BAD_ARGUMENT, NO_PAGE = 4, 8            # bits of the status word
+MOST_FORKED = 12800                     # sequences that fork_pages takes at once
 
 _status: dict = {}
 
@@ -150,6 +151,7 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     device, (in_pool, _, page, _, _) = k_pages.get_device(), k_pages.shape
     count, width, pages, scratch = _check_tables(table, refs, device)
     assert _is_ids(lengths, device, count) and _is_ids(parents, device, count) and pages == in_pool and width * page < 2 ** 31
+    assert count <= MOST_FORKED, "1 to 12800 sequences"
     status = device_status(k_pages.device) if status is None else status
     assert _is_ids(status, device, 1)
     table_out, lengths_out, refs_out = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refs)

@@ -288,6 +288,20 @@ def test_fork_compaction_and_reservation_of_large_tables(cuda_device):
     assert int(got[2]) == want[4]
 
 
+@pytest.mark.parametrize("width", [1, 4])
+@pytest.mark.parametrize("count", [3064, 3065, 3069, 12800])
+def test_fork_of_as_many_as_shared_memory_takes(cuda_device, count, width):
+    """Around the size from which a launch has to ask for more than it gets without asking, by one block and by a cluster; and the most."""
+    g = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 4 * width + 1, (count,), generator=g).tolist()
+    parents = torch.randint(-1, count, (count,), generator=g).tolist()
+    k, v, table, n, refs = plain.cache(lengths, 4, 1, 1, 8, BF16, seed=6, spare=count, width=width)
+    want = plain.fork(k, v, table, n, refs, parents, 4)
+    got = paged.fork_pages(k, v, table, n, refs, torch.tensor(parents, dtype=torch.int32, device="cuda"))
+    for a, b in zip((k, v, *got), want):
+        assert torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7))
+
+
 def test_fork_without_room_and_with_parents_that_are_none(cuda_device):
     lengths, page = [37, 20, 40], 16
     for parents, spare, bits in (([0, 0, 0], 0, 0), ([1, 1, 2], 0, 0), ([0, 0, 5], 1, 4), ([-2, 1, 1], 0, 12), ([2, 2, 2], 0, 0)):

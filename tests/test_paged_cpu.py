@@ -240,3 +240,12 @@ def test_reorder_refuses_more_rows_than_it_holds(calls):
     with pytest.raises(AssertionError, match="7000"):
         beam.reorder_states(on_gpu(torch.zeros(7001, 1)), on_gpu(torch.zeros(7001, dtype=I32)), status=status)
     assert not calls
+
+
+def test_forks_refuse_more_sequences_than_they_hold(calls):
+    many = lambda count: dict(table=torch.zeros(count, 1, dtype=I32), lengths=torch.zeros(count, dtype=I32), parents=torch.zeros(count, dtype=I32))  # noqa: E731
+    paged.fork_pages(**page_arguments(**many(12800)))
+    assert calls.pop()[1][15] == 12800
+    with pytest.raises(AssertionError, match="12800"):
+        paged.fork_pages(**page_arguments(**many(12801)))
+    assert not calls
