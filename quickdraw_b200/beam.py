@@ -30,7 +30,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     batch, beams, vocab = logits.shape
     device = logits.get_device()
     assert batch > 0 and 0 < beams <= MOST_BEAMS and vocab > 0 and batch * beams <= 65535, "1 to 32 beams"
-    assert logits.stride(2) == 1 and (batch == 1 or logits.stride(0) == beams * logits.stride(1)), "rows of contiguous logits, evenly apart"
+    apart = logits.stride(1) if beams > 1 else logits.stride(0)            # (of one beam or one group the stride says nothing)
+    assert logits.stride(2) == 1 and (batch == 1 or beams == 1 or logits.stride(0) == beams * apart), "rows of contiguous logits, evenly apart"
     assert scores.dtype is torch.float32 and scores.shape == (batch, beams) and scores.is_contiguous() and scores.get_device() == device
     if finished is not None:
         assert finished.dtype is torch.bool and finished.shape == (batch, beams) and finished.is_contiguous() and finished.get_device() == device
@@ -42,7 +43,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     parents, tokens = torch.empty_like(scores_out, dtype=torch.int32), torch.empty_like(scores_out, dtype=torch.long)
     size = scratch_size(device, "qd_beam_scratch_bytes", batch, beams, vocab, count)
     scratch = scores.new_empty(size // 4) if size else None
-    launch(logits, "qd_beam_select", ptr(logits), logits.stride(1) if beams > 1 else logits.stride(0), int(logits.dtype is torch.float32), ptr(scores),
+    launch(logits, "qd_beam_select", ptr(logits), apart, int(logits.dtype is torch.float32), ptr(scores),
            ptr(finished), 0 if finished is None else eos, ptr(scores_out), ptr(parents), ptr(tokens), ptr(scratch), batch, beams, vocab, count, int(placed))
     return scores_out, parents, tokens
 

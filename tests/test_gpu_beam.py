@@ -126,6 +126,16 @@ def test_rows_that_begin_anywhere(cuda_device, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [50, 5000])
+def test_single_beams_in_rows_apart(cuda_device, vocab, dtype):
+    whole = torch.full((6, vocab + 13), math.nan, dtype=dtype, device="cuda")
+    whole[:, :vocab] = (torch.randn((6, vocab), generator=torch.Generator().manual_seed(3)) * 3).to(dtype).cuda()
+    logits, scores = whole[:, :vocab].unsqueeze(1), torch.zeros((6, 1), device="cuda")
+    same(beam.beam_select(logits, scores), logits, scores)
+    same(beam.beam_select(logits, scores, candidates=5), logits, scores, candidates=5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("candidates", [1, 8, 32])
 @pytest.mark.parametrize("order", ["up", "down", "steps", "one in front"])
 def test_rows_in_order(cuda_device, order, candidates, dtype):

@@ -249,3 +249,12 @@ def test_forks_refuse_more_sequences_than_they_hold(calls):
     with pytest.raises(AssertionError, match="12800"):
         paged.fork_pages(**page_arguments(**many(12801)))
     assert not calls
+
+
+def test_select_takes_single_beams_in_rows_any_distance_apart(calls):
+    wide, scores = torch.zeros(5, 64), on_gpu(torch.zeros(5, 1))
+    for logits in (wide[:, :50].unsqueeze(1), wide[:, None, :50], wide.as_strided((5, 1, 50), (64, 7, 1))):
+        beam.beam_select(on_gpu(logits), scores)
+        assert calls.pop()[1][1] == 64
+    beam.beam_select(on_gpu(wide[:1, :50].unsqueeze(0).expand(1, 1, 50)), on_gpu(torch.zeros(1, 1)))
+    assert len(calls) == 1
