@@ -19,6 +19,7 @@ outside the tensors is touched.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 
@@ -68,6 +69,13 @@ def scratch_size(device: int, name: str, *sizes: int) -> int:
 
 def _is_ids(t, device, *shape) -> bool:
     return t.dtype is torch.int32 and t.shape == shape and t.get_device() == device and t.is_contiguous()
+
+
+def _endings(sequences, count: int, device) -> torch.Tensor:
+    """The parents of a fork in which the sequences of these numbers end and all others stay."""
+    ends = {operator.index(b) for b in sequences}            # (numbers of numpy and torch too, which need not be equal to their values in a set)
+    assert all(0 <= b < count for b in ends), "no such sequence"
+    return torch.tensor([-1 if b in ends else b for b in range(count)], dtype=torch.int32).to(device, non_blocking=True)
 
 
 def _check_pools(k, v):
@@ -229,9 +237,7 @@ class PagedCache:
 
     def free(self, sequences) -> None:
         """The sequences of these numbers end."""
-        ends = set(sequences)
-        assert all(0 <= b < self.sequences for b in ends), "no such sequence"
-        self.fork(torch.tensor([-1 if b in ends else b for b in range(self.sequences)], dtype=torch.int32).to(self.table.device, non_blocking=True))
+        self.fork(_endings(sequences, self.sequences, self.table.device))
 
     def compact(self) -> torch.Tensor:
         """The pages in use to the front (``compact_pages``); their number, on the device."""
@@ -334,9 +340,7 @@ class PagedBatchState:
 
     def free(self, sequences) -> None:
         """The sequences of these numbers end; their places are empty."""
-        ends = set(sequences)
-        assert all(0 <= b < self.batch for b in ends), "no such sequence"
-        self.fork(torch.tensor([-1 if b in ends else b for b in range(self.batch)], dtype=torch.int32).to(self.cache.table.device, non_blocking=True))
+        self.fork(_endings(sequences, self.batch, self.cache.table.device))
 
     def memory_bytes(self) -> int:
         return self.cache.memory_bytes() + self.rec_state.nbytes + self.conv_state.nbytes

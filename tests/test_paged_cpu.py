@@ -258,3 +258,19 @@ def test_select_takes_single_beams_in_rows_any_distance_apart(calls):
         assert calls.pop()[1][1] == 64
     beam.beam_select(on_gpu(wide[:1, :50].unsqueeze(0).expand(1, 1, 50)), on_gpu(torch.zeros(1, 1)))
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("several", [torch.tensor, lambda b: torch.tensor(b, dtype=I32).unbind(), lambda b: torch.tensor(b).numpy(), lambda b: (b[0], torch.tensor(b[1]))])
+def test_sequences_end_by_numbers_of_tensors(monkeypatch, several):
+    """A tensor's elements are not found in a set of whole numbers: nothing ended, without a word."""
+    cache, state = paged.PagedCache(1, 1, 8, 4, 4, 3, 8, "cpu"), paged.PagedBatchState(synthetic.model_config(num_layers=4, vocab_size=64), 3, 8, "cpu")
+    for of in (cache, state):
+        seen = []
+        monkeypatch.setattr(of, "fork", lambda parents, seen=seen: seen.append(parents.tolist()))
+        of.free(several([0, 2]))
+        assert seen == [[-1, 1, -1]]
+        with pytest.raises(AssertionError):
+            of.free(several([0, 3]))
+        with pytest.raises(TypeError):
+            of.free([0.5])
+        assert len(seen) == 1
