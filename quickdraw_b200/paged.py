@@ -31,21 +31,25 @@ BAD_ARGUMENT, NO_PAGE = 4, 8            # bits of the status word
 MOST_FORKED = 12800                     # sequences that fork_pages takes at once
 
 _status: dict = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_IN_CAPTURE = "a graph's memory is not shared: call device_status(device) before the capture, or give a status"
 
 
 def device_status(device) -> torch.Tensor:
-    """The status word of a device that calls without a word of their own share."""
+    """The status word of a device (without a number: of the current one) that calls without a word of their own share."""
     word = _status.get(device)
     if word is None:
-        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
-        assert not capturing, "a graph's memory is not shared: call device_status(device) before the capture, or give a status"
-        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        device = torch.device(device)
+        if device.type == "cuda":
+            if device.index is None:
+                return device_status(torch.device("cuda", _current_device()))
+            assert not torch.cuda.is_current_stream_capturing(), _IN_CAPTURE
+            with torch.cuda.device(device):
+                assert not torch.cuda.is_current_stream_capturing(), _IN_CAPTURE
+        word = _status.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))
         if device.type == "cuda":
             torch.cuda.current_stream(device).synchronize()         # any stream may use it from now on
     return word
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def launch(tensor: torch.Tensor, name: str, *args) -> None:

@@ -445,6 +445,15 @@ def test_forks_and_reservations_from_a_graph(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+def test_the_status_of_a_device_by_any_name(cuda_device):
+    table, lengths, refs = (torch.full(shape, fill, dtype=torch.int32, device="cuda") for shape, fill in (((1, 1), -1), ((1,), 0), ((1,), 1)))
+    word = paged.device_status(torch.device("cuda"))
+    word.zero_()
+    paged.reserve_pages(table, lengths, refs, 16)
+    assert int(paged.device_status("cuda")) == int(paged.device_status("cuda:0")) == int(word) == paged.NO_PAGE
+    word.zero_()
+
+
 def test_cache_through_its_life(cuda_device):
     """Rows written, sequences forked, ended, the pool compacted and resized: what every sequence sees stays the same."""
     page, layers, heads, dim = 16, 2, 2, 64

@@ -1,5 +1,6 @@
 """Refusals of the paged cache's and the beams' entry points, and what their drivers pass on, without a GPU."""
 
+import contextlib
 import math
 
 import pytest
@@ -209,7 +210,6 @@ def test_plain_forms_agree_with_themselves():
 
 def test_a_captured_step_is_not_replayed_after_a_resize(monkeypatch):
     """Its kernels have the addresses of pools whose memory was given back."""
-    import contextlib
     from types import SimpleNamespace
 
     from quickdraw_b200 import batch
@@ -274,3 +274,16 @@ def test_sequences_end_by_numbers_of_tensors(monkeypatch, several):
         with pytest.raises(TypeError):
             of.free([0.5])
         assert len(seen) == 1
+
+
+def test_a_device_has_one_status_however_it_is_named(monkeypatch):
+    zeros = torch.zeros
+    monkeypatch.setattr(paged, "_status", {})
+    monkeypatch.setattr(paged, "_current_device", lambda: 1)
+    monkeypatch.setattr(torch, "zeros", lambda *shape, device=None, **kwargs: zeros(*shape, **kwargs))
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: type("Stream", (), {"synchronize": lambda self: None})())
+    word = paged.device_status(torch.device("cuda", 1))
+    assert all(paged.device_status(device) is word for device in (torch.device("cuda"), "cuda", "cuda:1", torch.device("cuda:1")))
+    assert paged.device_status("cuda:0") is not word and paged.device_status("cpu") is paged.device_status(torch.device("cpu"))
