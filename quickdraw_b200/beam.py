@@ -108,21 +108,23 @@ def beam_search(decoder, prompts: list[list[int]], beams: int, max_tokens: int, 
     scores[:, 0] = 0.0                                     # all beams of a prompt are alike so far: one of them counts
     finished = torch.zeros((groups, beams), dtype=torch.bool, device=device)
     history = []
-    for step in range(max_tokens):
-        if graph:
-            _, logits = decoder.graph_step(tokens, state)
-        else:
-            _, logits = decoder.step(tokens, state, positions_checked=True)
-        scores, parents, chosen = beam_select(logits.view(groups, beams, -1), scores, finished=None if eos is None else finished, eos=eos)
-        tokens = chosen.view(-1)
-        history.append((parents.view(-1), tokens))
-        if eos is not None:
-            finished = finished.view(-1)[parents.view(-1).long()].view(groups, beams) | (chosen == eos)
-            if step % 16 == 15 and bool(finished.all()):
-                break
-        if step + 1 < max_tokens:
-            state.fork(parents.view(-1))
-    decoder.forget(state)
+    try:
+        for step in range(max_tokens):
+            if graph:
+                _, logits = decoder.graph_step(tokens, state)
+            else:
+                _, logits = decoder.step(tokens, state, positions_checked=True)
+            scores, parents, chosen = beam_select(logits.view(groups, beams, -1), scores, finished=None if eos is None else finished, eos=eos)
+            tokens = chosen.view(-1)
+            history.append((parents.view(-1), tokens))
+            if eos is not None:
+                finished = finished.view(-1)[parents.view(-1).long()].view(groups, beams) | (chosen == eos)
+                if step % 16 == 15 and bool(finished.all()):
+                    break
+            if step + 1 < max_tokens:
+                state.fork(parents.view(-1))
+    finally:
+        decoder.forget(state)                              # a captured step holds the pages; nobody else can drop it
     word = state.cache.check()
     assert word == 0, f"the search ran out of pages (status {word})"
     back, ids = torch.stack([p for p, _ in history]).tolist(), torch.stack([t for _, t in history]).tolist()

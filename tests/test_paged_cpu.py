@@ -287,3 +287,29 @@ def test_a_device_has_one_status_however_it_is_named(monkeypatch):
     word = paged.device_status(torch.device("cuda", 1))
     assert all(paged.device_status(device) is word for device in (torch.device("cuda"), "cuda", "cuda:1", torch.device("cuda:1")))
     assert paged.device_status("cuda:0") is not word and paged.device_status("cpu") is paged.device_status(torch.device("cpu"))
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_search_that_fails_leaves_no_captured_step(monkeypatch, graph):
+    class Decoder:
+        class ckpt:
+            config = synthetic.model_config(num_layers=4, vocab_size=64)
+        device = "cpu"
+        held: list = []
+
+        def graph_step(self, tokens, state, **kwargs):
+            self.held.append(state)
+            if len(self.held) == 3:
+                raise KeyboardInterrupt
+            return None, torch.zeros(4, 64)
+        step = graph_step
+
+        def forget(self, state):
+            self.held = [kept for kept in self.held if kept is not state]
+
+    decoder = Decoder()
+    monkeypatch.setattr(paged.PagedBatchState, "fork", lambda self, parents: None)
+    monkeypatch.setattr(beam, "beam_select", lambda logits, scores, **kwargs: (scores, torch.zeros(2, 2, dtype=I32), torch.zeros(2, 2, dtype=torch.long)))
+    with pytest.raises(KeyboardInterrupt):
+        beam.beam_search(decoder, [[1], [2]], 2, 9, graph=graph)
+    assert decoder.held == []
