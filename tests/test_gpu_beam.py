@@ -126,6 +126,18 @@ def test_rows_that_begin_anywhere(cuda_device, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch,beams,vocab", [(2, 32, 2049), (1, 32, 70001), (3, 31, 6151), (2, 17, 66000)])
+def test_many_beams_of_long_rows(cuda_device, batch, beams, vocab, dtype):
+    """The most lists that a group's blocks join, from two pieces a row to thirty-two; scores near one another, so that many beams count."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = (torch.randn((batch, beams, vocab), generator=g) * 3).to(dtype).cuda()
+    scores = (torch.randn((batch, beams), generator=g) * 0.5 - 10).cuda()
+    finished = torch.rand((batch, beams), generator=g).cuda() < 0.2
+    for kwargs in (dict(), dict(candidates=32), dict(finished=finished, eos=vocab - 1), dict(finished=finished, eos=0, candidates=32)):
+        same(beam.beam_select(logits, scores, **kwargs), logits, scores, **kwargs)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("vocab", [50, 5000])
 def test_single_beams_in_rows_apart(cuda_device, vocab, dtype):
     whole = torch.full((6, vocab + 13), math.nan, dtype=dtype, device="cuda")

@@ -134,6 +134,16 @@ def test_infinite_and_largest_values(cuda_device, heads, kv_heads, dim, dtype):
             assert bool(((got - want).abs() <= bound)[:, :, columns].all()), (lengths, seen)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (4, 2, 64), (24, 2, 128)])
+def test_attention_over_pages_that_sequences_share(cuda_device, heads, kv_heads, dim, dtype):
+    """Beams behind a common beginning, as forks leave them: 700 rows of the first sequence in all tables, then rows of their own."""
+    *args, gate = problem([777, 777, 703, 720, 300, 777], heads, kv_heads, dim, 20, dtype, seed=4, gate=True, shared=35)
+    assert int((args[3] == args[3][:1]).sum(0)[:15].min()) == 6                  # one page in six tables
+    check(paged.paged_attention(*args, gate=gate), *args, gate=gate)
+    check(paged.paged_attention(*args, gate=gate, window=100, sinks=30), *args, gate=gate, window=100, sinks=30)
+
+
 def test_views_with_other_strides(cuda_device):
     """Layers of one pool, pools with the heads outside of the rows, queries and gates inside a projection, a table inside a larger one."""
     lengths, page = [120, 77, 300], 16
