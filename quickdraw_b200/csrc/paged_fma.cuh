@@ -99,7 +99,7 @@ template <int D, int HEADS> struct PagedFma {
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            x[s] = weight_of(x[s], m);
+            x[s] = weight_of(x[s], m) * kPagedWeight;
             l += x[s];
             if (kAtOnce > 1 && lane % kLanes < HEADS)
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(weights + ((s * kAtOnce + part) * 8 + own) * 4), "f"(x[s]) : "memory");
@@ -126,26 +126,10 @@ template <int D, int HEADS> struct PagedFma {
                 for (int j = 0; j < 4; ++j) acc[h][j] = fma2(make_float2(w[h], w[h]), v[j], acc[h][j]);
         }
     }
-    QD_DEVINL bool unbounded() const {
-        float odd = 0.f;                                               // zero times what is not finite is NaN
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) odd = fmaf(acc[h][j].x, 0.f, fmaf(acc[h][j].y, 0.f, odd));
-        return odd != 0.f;
-    }
     QD_DEVINL void leave(int, float* state, float2* stats) {
 #pragma unroll
-        for (int e = kLanes; e < 32; e <<= 1) l += __shfl_xor_sync(0xffffffffu, l, e);
-        const float inverse = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            const float of = __shfl_sync(0xffffffffu, inverse, lane_of(h));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[h][j] = mul2(acc[h][j], make_float2(of, of));
-        }
-#pragma unroll
         for (int e = kLanes; e < 32; e <<= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, e);
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
 #pragma unroll

@@ -26,8 +26,8 @@ QD_DEVINL uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
 }
-QD_DEVINL float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
-QD_DEVINL float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+QD_DEVINL uint32_t high_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+QD_DEVINL float rest_of(float x) { return fmaxf(x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), x * 0x1p-20f); }
 
 template <int D, int NT> struct PagedMma {
     using Type = bf16;
@@ -107,15 +107,14 @@ template <int D, int NT> struct PagedMma {
                 for (int d = 0; d < D / 16; ++d) { acc[n][d][0] *= fix0; acc[n][d][1] *= fix1; acc[n][d][2] *= fix0; acc[n][d][3] *= fix1; }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = weight_of(x[e], m[n][e & 1]);
+            for (int e = 0; e < 4; ++e) x[e] = weight_of(x[e], m[n][e & 1]) * kPagedWeight;
             l[n][0] += x[0] + x[2];
             l[n][1] += x[1] + x[3];
-            // weights in two bf16 pieces (sixteen bits): one alone would be off by as much as the result's own rounding (of an infinite
-            // value they may make NaN: such sums are formed again)
-            const uint32_t h0 = pack2(x[0], x[1]), h1 = pack2(x[2], x[3]);
-            hi[n][0] = transposed(h0); hi[n][1] = transposed(h1);
-            lo[n][0] = transposed(pack2(x[0] - low_of(h0), x[1] - high_of(h0)));
-            lo[n][1] = transposed(pack2(x[2] - low_of(h1), x[3] - high_of(h1)));
+            // weights in two bf16 pieces (sixteen bits): one alone would be off by as much as the result's own rounding.  The first is cut off, not rounded,
+            // and the second is at least 2^-20 of the weight: zero or a negative number times an infinite value would make NaN of an infinite mean
+            hi[n][0] = transposed(high_halves(x[0], x[1])); hi[n][1] = transposed(high_halves(x[2], x[3]));
+            lo[n][0] = transposed(pack2(rest_of(x[0]), rest_of(x[1])));
+            lo[n][1] = transposed(pack2(rest_of(x[2]), rest_of(x[3])));
         }
     }
     QD_DEVINL void values(uint32_t values) {
@@ -130,16 +129,6 @@ template <int D, int NT> struct PagedMma {
             }
         });
     }
-    QD_DEVINL bool unbounded() const {
-        float odd = 0.f;                                               // zero times what is not finite is NaN
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd = fmaf(acc[n][d][e], 0.f, odd);
-        return odd != 0.f;
-    }
     QD_DEVINL void leave(int n, float* state, float2* stats) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -147,11 +136,10 @@ template <int D, int NT> struct PagedMma {
             for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
             const int h = 2 * t + e;
             if (g == 0) stats[h] = make_float2(m[n][e], l[n][e]);
-            const float inverse = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-                for (int up = 0; up < 2; ++up) state[h * D + ((d * 16 + up * 8 + g) ^ (t << 3))] = acc[n][d][2 * up + e] * inverse;
+                for (int up = 0; up < 2; ++up) state[h * D + ((d * 16 + up * 8 + g) ^ (t << 3))] = acc[n][d][2 * up + e];
         }
     }
 };

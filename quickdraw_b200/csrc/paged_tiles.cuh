@@ -1,6 +1,6 @@
 // Attention over pages, a tile of positions at a time: who works on what, and how the tiles come.  What is done with a tile is given by a class Work:
 //   Type, kDim (columns, at least the head dimension), kHeads (query heads, a multiple of eight), kTile (positions), kWarps, kAhead (tiles on their way),
-//   kSeqs (sequences of a launch), begin(queries), scores(keys, rows, scale), values(values), unbounded() (a sum is not finite), leave(n, state, stats).
+//   kSeqs (sequences of a launch), begin(queries), scores(keys, rows, scale), values(values), leave(n, state, stats).
 #pragma once
 #include "paged.cuh"
 
@@ -23,6 +23,16 @@ QD_DEVINL void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memo
 template <int N> QD_DEVINL void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // exp2 of a difference to a running maximum that may be -inf (nothing seen yet)
 QD_DEVINL float weight_of(float s, float top) { return exp2f(s - (top == -INFINITY ? 0.f : top)); }
+// What weights are taken times.  They are up to 2^8 (see the Work): the sum of as many as a warp meets (2^24) times the largest value stays below the
+// largest number, and what is joined after it are means.  (Of values below 2^-94 bits are lost instead.)
+constexpr float kPagedWeight = 0x1p-32f;
+
+// 1 / x of a normal number, off by 2^-23 at most
+QD_DEVINL float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Four or eight elements from a place that may not be on a 16-byte boundary.
 QD_DEVINL uint4 paged_load16(const float* src) {
@@ -54,44 +64,6 @@ template <class W> struct PagedTiles {
     static constexpr int kStride = kPagedGroup * W::kTile, kLook = 32 / W::kTile;      // between two tiles of a warp; tiles of a look into the table
     static_assert(8 * W::kDim * 4 <= kSlot, "eight heads' state fits the slot that is free");
 };
-
-// What a warp leaves of eight heads (from the n-th eight) where one of its sums is not finite: an infinite value has met a weight's piece that is zero or
-// negative, or the sum of large values has passed the largest number (weights are up to 2^8, their sum up to the number of rows times that).  Formed again,
-// a position at a time with whole weights, as a mean from the first row on, which is no larger than the largest value.  Slow and next to
-// never needed: 32 sequences of 8192 positions, 16 heads on 2 of 256, take 96 us, 1.7 ms with one infinity and 7.3 ms with one in every eighth row.
-template <class W>
-QD_DEVINL void paged_again(const PagedParams& p, const Piece& a, int among, int n, float* state, float2* stats) {
-    using T = typename W::Type;
-    constexpr int D = W::kDim;
-    const int lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int h = 0; h < 8 && n * 8 + h < a.heads; ++h) {
-        const T* query = (const T*)p.q + a.b * p.q_row + (a.head0 + n * 8 + h) * p.q_head;
-        float m = -INFINITY, l = 0.f, mean[D / 32] = {};
-#pragma unroll 1
-        for (int i = a.t0 + among * W::kTile, in = 0; i < a.t1; in = in == W::kTile - 1 ? 0 : in + 1, i += in ? 1 : PagedTiles<W>::kStride - W::kTile + 1) {
-            const int position = paged_position(p, i, a.skip), entry = __ldcg(p.table + a.b * p.table_stride + position / p.page);
-            if (entry < 0 || entry >= p.pages) continue;
-            const long long off = entry * p.page_stride + position % p.page * p.row_stride + a.kvh * p.head_stride;
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-                if (j * 32 + lane < p.dim) s += paged_load(query + j * 32 + lane) * paged_load((const T*)p.k + off + j * 32 + lane);
-            s = warp_sum(s) * p.scale;
-            const float top = fmaxf(m, s), w = weight_of(s, top), before = l * weight_of(m, top);
-            m = top;
-            l = before + w;
-            if (l == 0.f) continue;                                         // scores of -inf alone
-            const float now = w / l, then = before / l;
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-                if (j * 32 + lane < p.dim) mean[j] = mean[j] * then + now * paged_load((const T*)p.v + off + j * 32 + lane);
-        }
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) state[h * D + ((j * 32 + lane) ^ ((h >> 1) << 3))] = mean[j];
-        if (lane == 0) stats[h] = make_float2(m, l);
-    }
-}
 
 template <class W>
 __global__ void __launch_bounds__(PagedTiles<W>::kThreads, 1) paged_tiles_kernel(const PagedParams p) {
@@ -229,15 +201,12 @@ __global__ void __launch_bounds__(PagedTiles<W>::kThreads, 1) paged_tiles_kernel
         }
         // the next queries came with the first tile that this part sent for: behind more tiles than are on their way they have been waited for
         if (a.t1 - a.t0 <= (W::kAhead * kPagedGroup + among) * W::kTile) cp_async_wait_all();
-        // ---- the four states (weighted means, so that no join passes the largest number), eight heads at a time, each in the slot that its warp has free:
-        // [head][column], columns of heads 2 t and 2 t + 1 turned by 8 t (four heads' columns meet 32 banks)
+        // ---- the four states, eight heads at a time, each in the slot that its warp has free: [head][column], columns of heads 2 t and 2 t + 1 turned by
+        // 8 t (four heads' columns meet 32 banks); joined to means, no larger than the largest value
         if (lane == 0) freed[warp] = (uint8_t)free_slot();
-        const bool again = __any_sync(0xffffffffu, work.unbounded());
 #pragma unroll
         for (int n = 0; n < W::kHeads / 8; ++n) {
-            float* state = reinterpret_cast<float*>(own + free_slot() * S::kSlot);
-            if (again) paged_again<W>(p, a, among, n, state, stats + among * W::kHeads + n * 8);
-            else work.leave(n, state, stats + among * W::kHeads + n * 8);
+            work.leave(n, reinterpret_cast<float*>(own + free_slot() * S::kSlot), stats + among * W::kHeads + n * 8);
             meet();
 #pragma unroll
             for (int i = among * 32 + lane; i < 8 * (D / 4); i += kPagedGroup * 32) {
@@ -248,21 +217,21 @@ __global__ void __launch_bounds__(PagedTiles<W>::kThreads, 1) paged_tiles_kernel
 #pragma unroll
                 for (int w = 0; w < kPagedGroup; ++w) { of[w] = stats[w * W::kHeads + h]; top = fmaxf(top, of[w].x); }
 #pragma unroll
-                for (int w = 0; w < kPagedGroup; ++w) { of[w].x = of[w].y == 0.f ? 0.f : exp2f(of[w].x - top) * of[w].y; den += of[w].x; }
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                const float inverse = den == 0.f ? 0.f : 1.f / den;
+                for (int w = 0; w < kPagedGroup; ++w) { of[w].x = of[w].y == 0.f ? 0.f : exp2f(of[w].x - top); den += of[w].x * of[w].y; }
+                float4 mean = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float inverse = den == 0.f ? 0.f : reciprocal(den);
 #pragma unroll
                 for (int w = 0; w < kPagedGroup; ++w) {
                     const float share = of[w].x * inverse;
                     const int other = group * kPagedGroup + w;
                     const float4 v = *reinterpret_cast<const float4*>(paged_smem + other * S::kRing + freed[other] * S::kSlot + place * 4);
-                    sum.x += share * v.x; sum.y += share * v.y; sum.z += share * v.z; sum.w += share * v.w;
+                    mean.x += share * v.x; mean.y += share * v.y; mean.z += share * v.z; mean.w += share * v.w;
                 }
                 if (p.cuts.most) {
-                    *reinterpret_cast<float4*>(p.partial + paged_place(p, a, h) * p.dim + f) = sum;
+                    *reinterpret_cast<float4*>(p.partial + paged_place(p, a, h) * p.dim + f) = mean;
                     if (f == 0) p.stats[paged_place(p, a, h)] = make_float2(top, den);
                 } else {
-                    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+                    const float v[4] = {mean.x, mean.y, mean.z, mean.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) paged_put<T>(p, a.b, a.head0 + h, f + e, v[e]);
                 }

@@ -144,6 +144,21 @@ def test_attention_over_pages_that_sequences_share(cuda_device, heads, kv_heads,
     check(paged.paged_attention(*args, gate=gate, window=100, sinks=30), *args, gate=gate, window=100, sinks=30)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_largest_values_under_scores_that_rise(cuda_device, dtype):
+    """A softmax's reference may lie 2^8 below its scores: weights of 256, and many of them, times the largest numbers."""
+    largest = 3.3e38
+    for heads, kv_heads, dim in ((16, 2, 256), (32, 1, 128), (4, 2, 64)):
+        q, k, v, table, n, _ = problem([5000, 200, 60], heads, kv_heads, dim, 16, dtype)
+        q.fill_(1.0)
+        for b, count in enumerate((5000, 200, 60)):
+            p = torch.arange(count, device="cuda")
+            k[table[b, p // 16].long(), p % 16] = (torch.clamp(p / 40, max=5.25) / dim).to(dtype)[:, None, None]
+            v[table[b, p // 16].long(), p % 16] = largest
+            v[table[b, p // 16].long(), p % 16, :, dim // 2:] = -largest
+        check(paged.paged_attention(q, k, v, table, n, scale=1.0), q, k, v, table, n, scale=1.0)
+
+
 def test_views_with_other_strides(cuda_device):
     """Layers of one pool, pools with the heads outside of the rows, queries and gates inside a projection, a table inside a larger one."""
     lengths, page = [120, 77, 300], 16
