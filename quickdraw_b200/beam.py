@@ -78,8 +78,10 @@ def beam_search(decoder, prompts: list[list[int]], beams: int, max_tokens: int, 
     """The ``beams`` best answers to every prompt, each (token ids, EOS included; log-probability / length ** length_penalty), best first.
 
     ``decoder`` is a ``BatchDecode``; all beams of all prompts are one batch.  The beams of a prompt share the pages of what they have in
-    common; a step appends a token to every beam, chooses, and forks the state by the parents, all without waiting for the
-    device.  ``graph``: the step replayed from a CUDA graph (``BatchDecode.graph_step``)."""
+    common; a step appends a token to every beam, chooses, and forks the state by the parents.  The host waits for the device only
+    where ``eos`` is given, every sixteenth step, to see whether all have ended.  The choice goes by the log-probability alone, of
+    beams that have ended as of the others: ``length_penalty`` orders the answers that are left at the end.  ``graph``: the step
+    replayed from a CUDA graph (``BatchDecode.graph_step``)."""
     config = decoder.ckpt.config
     assert prompts and all(len(p) > 0 for p in prompts), "at least one prompt of at least one token"
     assert 1 <= beams <= MOST_BEAMS and max_tokens >= 0, "1 to 32 beams"

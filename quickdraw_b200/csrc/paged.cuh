@@ -54,7 +54,7 @@ QD_DEVINL float2 fma2(float2 a, float2 b, float2 c) {
 // its result does not depend on its neighbours: as if all of the batch were as long, so that they fill some rounds of workers in least time (a part
 // costs `kPagedFixed` units beside its own: its state is written, read and joined); of cuts that are within 1 / 16 of it the finest, because beside
 // other lengths smaller parts are shared out more evenly.
-constexpr int kPagedCuts = 6, kPagedLeast = 1;
+constexpr int kPagedCuts = 6;
 constexpr float kPagedFixed = 1.f;
 // parts of a sequence (their reciprocal), rounds of workers; the most parts of any, 0: one each, whose results the parts' kernel writes itself
 struct PagedCuts { float each[kPagedCuts], rounds[kPagedCuts]; int most; };
@@ -82,7 +82,7 @@ static __device__ __forceinline__ int paged_parts(const PagedCuts& c, int seen, 
     float per[kPagedCuts], cost[kPagedCuts], least = INFINITY;
 #pragma unroll
     for (int i = 0; i < kPagedCuts; ++i) {
-        per[i] = fmaxf(ceilf((float)n * c.each[i]), (float)kPagedLeast);
+        per[i] = ceilf((float)n * c.each[i]);
         cost[i] = c.rounds[i] * (per[i] + kPagedFixed);
         least = fminf(least, cost[i]);
     }

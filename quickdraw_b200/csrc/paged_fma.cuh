@@ -11,7 +11,7 @@ namespace qd {
 template <int D, int HEADS> struct PagedFma {
     using Type = float;
     static constexpr int kDim = D, kHeads = 8, kTile = 8, kSeqs = 256;
-    static constexpr bool kNarrow = D == 64 && HEADS == 4;               // state and queries fit 128 registers: 28.2 us of the first, 29.4 by eight warps, 8 on 8 of 64 (370 MB) 73 and 80; eight heads of 64 would not, 79 for 35
+    static constexpr bool kNarrow = D == 64 && HEADS == 4;               // state and queries fit 128 registers but for five words: 28.2 us of the first, 29.4 by eight warps, 8 on 8 of 64 (370 MB) 73 and 80; eight heads of 64 would not, 79 for 35
     static constexpr int kWarps = kNarrow ? 16 : 8, kAhead = D == 256 ? 1 : D == 128 || kNarrow ? 2 : 4;
     static constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kSteps = kTile / kAtOnce;        // lanes of a position, positions at once
     static constexpr int kSpare = kAtOnce > 1 ? kTile * 8 * 4 : 0;

@@ -35,7 +35,7 @@ template <int D, int NT> struct PagedMma {
     static constexpr int kSeqs = D == 256 && NT == 2 ? 192 : 1024;     // (what memory has room for)
     const int lane, g, t;
     const uint32_t key_turn, value_turn;
-    static constexpr bool kHeld = NT == 1 || D == 128;                 // queries in registers (24 heads of 128 on a key head, 28 x 12307 positions: 122.7 us, 130.5 read for each tile); sixteen heads of 64 or 256 find no room
+    static constexpr bool kHeld = NT == 1 || D == 128;                 // queries in registers (24 heads of 128 on a key head, 28 x 12307 positions: 122.7 us, 130.5 read for each tile); sixteen heads of 64 (five words lie outside of the registers as it is) or 256 find no room
     uint32_t q_row, q4[kHeld ? NT * D / 32 : 1][4];
     float acc[NT][D / 16][4], m[NT][2], l[NT][2];                      // columns g and g + 8 of every sixteen, heads 2 t and 2 t + 1
     uint32_t hi[NT][2], lo[NT][2];

@@ -11,7 +11,9 @@ the front).  ``PagedCache`` holds the tensors of several layers; ``PagedBatchSta
 for ``BatchDecode`` that can be forked (beam search, several answers to one prompt), whose pages need no more memory than
 the tokens in it.
 
-All of it stays on the device and can be captured; calls go to the current stream of the tensors' device.  What only the device
+The functions stay on the device and can be captured, and so do ``reserve``, ``fork``, ``compact``, ``write`` and ``read``; ``free`` and
+``admit`` take their numbers from the host (not in a capture), ``resize``, ``extract`` and ``check`` wait for it.  Calls go to the
+current stream of the tensors' device.  What only the device
 knows (a pool without a free page, a parent that is no sequence) sets bits of a status word, ``PagedCache.check``; nothing
 outside the tensors is touched.
 """
@@ -276,7 +278,8 @@ class PagedCache:
                ptr(self.table[b]), ptr(self.status), layers, self.table.shape[1], pages, page, first, count, int(out))
 
     def write(self, b: int, k: torch.Tensor, v: torch.Tensor, first: int, count: int) -> None:
-        """Rows first .. first + count - 1 of sequence b, whose pages are set aside, from k, v [layers, >= count, kv_heads, head_dim]."""
+        """Rows first .. first + count - 1 of sequence b, whose pages are set aside, from k, v [layers, >= count, kv_heads, head_dim].  Rows of
+        pages that it shares are theirs too who share them."""
         self._rows(b, k, v, first, count, False)
 
     def read(self, b: int, k: torch.Tensor, v: torch.Tensor, first: int, count: int) -> None:
