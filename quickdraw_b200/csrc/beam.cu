@@ -64,7 +64,7 @@ QD_DEVINL unsigned long long warp_sorted(unsigned long long key, int lane) {
 // above it; it rises to the candidates-th of the list when that grows.  32 x 8 rows of 151936 with the merge: 40 us fp32 (156 MB; 35 with no keys
 // and no exponentials to take) and 40 bf16; fp32 43 with the next chunk in registers (fewer blocks an SM) and a second barrier in every chunk that
 // has a key.  Two chunks ahead took 42 (fewer blocks), a warp with a list of its own ten more (eight first chunks instead of one), 256 threads seven more.
-// 4 x 32 rows: 65 us, 98 with a first bound from each warp alone (a fifth of the chunk is above it).
+// 4 x 32 rows: 65 to 68 us, 98 with a first bound from each warp alone (a fifth of the chunk is above it).
 constexpr int kPartThreads = 128, kPartEach = 16, kPartMany = 32, kPartPending = 16, kPartSlack = 4;
 template <typename T> constexpr size_t part_ring() { return 2 * kPartThreads * kPartEach * sizeof(T); }
 template <typename T>
