@@ -79,6 +79,8 @@ def _is_ids(t, device, *shape) -> bool:
 
 def _endings(sequences, count: int, device) -> torch.Tensor:
     """The parents of a fork in which the sequences of these numbers end and all others stay."""
+    sequences = list(sequences)
+    assert not any(isinstance(b, bool) or getattr(b, "dtype", None) is torch.bool for b in sequences), "numbers of sequences, not a mask"
     ends = {operator.index(b) for b in sequences}            # (numbers of numpy and torch too, which need not be equal to their values in a set)
     assert all(0 <= b < count for b in ends), "no such sequence"
     return torch.tensor([-1 if b in ends else b for b in range(count)], dtype=torch.int32).to(device, non_blocking=True)

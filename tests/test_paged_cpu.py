@@ -313,3 +313,12 @@ def test_a_search_that_fails_leaves_no_captured_step(monkeypatch, graph):
     with pytest.raises(KeyboardInterrupt):
         beam.beam_search(decoder, [[1], [2]], 2, 9, graph=graph)
     assert decoder.held == []
+
+
+@pytest.mark.parametrize("mask", [[True, False, True], torch.tensor([True, False, True]), torch.tensor([True, False, True]).numpy()])
+def test_sequences_do_not_end_by_a_mask(monkeypatch, mask):
+    """True and False are 1 and 0 as numbers: other sequences than meant would end."""
+    cache = paged.PagedCache(1, 1, 8, 4, 4, 3, 8, "cpu")
+    monkeypatch.setattr(cache, "fork", lambda parents: pytest.fail("ended"))
+    with pytest.raises((AssertionError, TypeError)):
+        cache.free(mask)
